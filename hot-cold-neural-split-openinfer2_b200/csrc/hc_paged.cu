@@ -1,0 +1,898 @@
+// Paged 8-bit key/value cache: block tables and slot maps from request
+// lengths, rotary positions, and the write of a step's keys and values.
+//
+// A page holds page_size tokens of every key-value head,
+// [n_kv_heads][page_size][head_dim] e4m3 bytes, with one power-of-two scale
+// per page and head: value = byte * scale.  e4m3 is a floating-point format,
+// so a power of two costs no precision over absmax / 448; it makes the
+// division exact (one rounding in all) and lets a page that grows be rescaled
+// without a second rounding, except of values that fall among the format's
+// subnormals.
+#include <cooperative_groups.h>
+
+#include "hc_common.cuh"
+
+namespace hcp {
+using namespace hc;
+namespace cg = cooperative_groups;
+
+constexpr int MAX_REQ = 2048;           // requests of one step (their offsets sit in shared memory)
+constexpr int PLAN_THREADS = 1024;
+constexpr int PLAN_CL = 8;              // CTAs of a plan with many rows (one cluster)
+
+// ---------------------------------------------------------------------------
+// page plan
+// ---------------------------------------------------------------------------
+struct PlanArgs {
+  const int32_t* starts;
+  const int32_t* q_lens;
+  int n_req;
+  int32_t* tables;
+  int64_t stride;
+  int width;
+  const int32_t* free_pages;
+  int n_pages;
+  int32_t* n_free;
+  int page_size, n_rows;
+  int32_t* cu_q;
+  int32_t* kv_lens;
+  int64_t* positions;
+  int64_t* slots;
+  int32_t* status;
+};
+
+// inclusive sums of two values over the block (1024 threads)
+__device__ __forceinline__ void block_scan2(int64_t& a, int64_t& b, int64_t (*wsum)[2]) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o);
+    if (lane >= o) {
+      a += x;
+      b += y;
+    }
+  }
+  if (lane == 31) {
+    wsum[w][0] = a;
+    wsum[w][1] = b;
+  }
+  __syncthreads();
+  if (w == 0) {
+    int64_t x = wsum[lane][0], y = wsum[lane][1];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t p = __shfl_up_sync(0xffffffffu, x, o), q = __shfl_up_sync(0xffffffffu, y, o);
+      if (lane >= o) {
+        x += p;
+        y += q;
+      }
+    }
+    wsum[lane][0] = x;
+    wsum[lane][1] = y;
+  }
+  __syncthreads();
+  if (w > 0) {
+    a += wsum[w - 1][0];
+    b += wsum[w - 1][1];
+  }
+}
+
+// first negative entry of row[lo..hi), whose filled entries form a prefix; hi if there is none
+__device__ __forceinline__ int first_missing(const int32_t* row, int lo, int hi) {
+  if (lo >= hi) return hi;
+  const int32_t a = row[lo], b = row[hi - 1];
+  if (a < 0) return lo;
+  if (b >= 0) return hi;
+  while (hi - lo > 1) {                 // row[lo] filled, row[hi - 1] missing
+    const int mid = lo + (hi - lo) / 2;
+    if (row[mid] < 0) hi = mid;
+    else lo = mid;
+  }
+  return hi;
+}
+
+// largest i in [0, n) with first[i] <= x (first[0] = 0, ascending)
+__device__ __forceinline__ int owner(const int32_t* first, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (first[mid] <= x) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// Every CTA of the cluster computes the same two prefix sums over the requests
+// (new rows, pages to take), so nothing is exchanged; a cluster barrier keeps
+// the tables and the free count unchanged until every CTA has read them.
+// Latency-bound: 8 n_req + 16 n_rows bytes.
+__global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const PlanArgs p) {
+  __shared__ int32_t s_cu[MAX_REQ + 1], s_take[MAX_REQ + 1], s_first[MAX_REQ], s_start[MAX_REQ];
+  __shared__ int64_t wsum[32][2];
+  __shared__ int s_bad;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int t = threadIdx.x, ncta = gridDim.x, cta = blockIdx.x;
+  const int per = (p.n_req + PLAN_THREADS - 1) / PLAN_THREADS;       // 1 or 2 requests a thread
+  const int n_free = *p.n_free;
+  if (t == 0) s_bad = n_free < 0 || n_free > p.n_pages;
+  __syncthreads();
+  int64_t rows = 0, take = 0;
+  bool bad = false;
+  for (int i = 0; i < per; ++i) {
+    const int r = t * per + i;
+    if (r >= p.n_req) break;
+    const int start = p.starts[r], q = p.q_lens[r];
+    const int64_t end = (int64_t)start + q;
+    int first = 0, miss = 0;
+    if (start < 0 || q < 0 || end > (int64_t)p.width * p.page_size) {
+      bad = true;
+    } else {
+      const int lo = start / p.page_size, hi = q ? ((int)end - 1) / p.page_size + 1 : lo;
+      first = first_missing(p.tables + r * p.stride, lo, hi);
+      miss = hi - first;
+      rows += q;
+      take += miss;
+    }
+    s_start[r] = start;
+    s_first[r] = first;
+    s_cu[r] = q;                      // lengths for now
+    s_take[r] = miss;
+  }
+  if (bad) s_bad = 1;
+  int64_t rows_in = rows, take_in = take;
+  block_scan2(rows_in, take_in, wsum);
+  const int64_t total_rows = wsum[31][0], total_take = wsum[31][1];
+  bad = s_bad || total_rows > p.n_rows || total_take > n_free;
+  if (!bad) {
+    int64_t a = rows_in - rows, b = take_in - take;
+    for (int i = 0; i < per; ++i) {
+      const int r = t * per + i;
+      if (r >= p.n_req) break;
+      const int q = s_cu[r], m = s_take[r];
+      s_cu[r] = (int32_t)a;
+      s_take[r] = (int32_t)b;
+      a += q;
+      b += m;
+    }
+  }
+  if (t == 0 && !bad) {
+    s_cu[p.n_req] = (int32_t)total_rows;
+    s_take[p.n_req] = (int32_t)total_take;
+  }
+  __syncthreads();
+  if (ncta > 1) cluster.sync();       // every CTA has read what is written below
+  const int lane0 = cta * PLAN_THREADS + t, lanes = ncta * PLAN_THREADS;
+  if (bad) {                          // nothing allocated, no rows
+    if (lane0 == 0 && p.status) atomicOr(p.status, HC_ERR_RANGE);
+    for (int r = lane0; r <= p.n_req; r += lanes) {
+      p.cu_q[r] = 0;
+      if (r < p.n_req) p.kv_lens[r] = p.starts[r];
+    }
+    for (int i = lane0; i < p.n_rows; i += lanes) {
+      p.positions[i] = -1;
+      p.slots[i] = -1;
+    }
+    return;
+  }
+  for (int r = lane0; r <= p.n_req; r += lanes) {
+    p.cu_q[r] = s_cu[r];
+    if (r < p.n_req) p.kv_lens[r] = s_start[r] + s_cu[r + 1] - s_cu[r];
+  }
+  bool stray = false;
+  for (int m = lane0; m < (int)total_take; m += lanes) {
+    const int r = owner(s_take, p.n_req, m);
+    const int32_t page = p.free_pages[n_free - 1 - m];
+    stray |= page < 0 || page >= p.n_pages;
+    p.tables[r * p.stride + s_first[r] + m - s_take[r]] = page;
+  }
+  for (int i = lane0; i < p.n_rows; i += lanes) {
+    int64_t pos = -1, slot = -1;
+    if (i < (int)total_rows) {
+      const int r = owner(s_cu, p.n_req, i);
+      const int at = s_start[r] + (i - s_cu[r]);
+      const int pg = at / p.page_size;
+      pos = at;
+      const int32_t page = pg < s_first[r] ? p.tables[r * p.stride + pg]
+                                           : p.free_pages[n_free - 1 - (s_take[r] + pg - s_first[r])];
+      if (page < 0 || page >= p.n_pages) stray = true;
+      else slot = (int64_t)page * p.page_size + at % p.page_size;
+    }
+    p.positions[i] = pos;
+    p.slots[i] = slot;
+  }
+  if (stray && p.status) atomicOr(p.status, HC_ERR_RANGE);
+  if (lane0 == 0) *p.n_free = n_free - (int)total_take;
+}
+
+struct ReleaseArgs {
+  const uint8_t* done;
+  int n_req;
+  int32_t* tables;
+  int64_t stride;
+  int width;
+  int32_t* free_pages;
+  int n_pages;
+  int32_t* n_free;
+  int32_t* status;
+};
+
+// The pages of the finished requests go back onto the stack, request order
+// then page order.  One CTA: a serving step releases a few requests.
+__global__ void __launch_bounds__(PLAN_THREADS) page_release_kernel(const ReleaseArgs p) {
+  __shared__ int32_t s_put[MAX_REQ + 1];
+  __shared__ int64_t wsum[32][2];
+  __shared__ int s_bad;
+  const int t = threadIdx.x;
+  const int per = (p.n_req + PLAN_THREADS - 1) / PLAN_THREADS;
+  const int n_free = *p.n_free;
+  if (t == 0) s_bad = n_free < 0 || n_free > p.n_pages;
+  __syncthreads();
+  int64_t put = 0, unused = 0;
+  for (int i = 0; i < per; ++i) {
+    const int r = t * per + i;
+    if (r >= p.n_req) break;
+    const int n = p.done[r] ? first_missing(p.tables + r * p.stride, 0, p.width) : 0;
+    s_put[r] = n;
+    put += n;
+  }
+  int64_t in = put;
+  block_scan2(in, unused, wsum);
+  const int64_t total = wsum[31][0];
+  int64_t a = in - put;
+  for (int i = 0; i < per; ++i) {
+    const int r = t * per + i;
+    if (r >= p.n_req) break;
+    const int n = s_put[r];
+    s_put[r] = (int32_t)min(a, (int64_t)INT32_MAX);
+    a += n;
+  }
+  const bool over = n_free + total > p.n_pages;
+  if (t == 0) s_put[p.n_req] = over ? 0 : (int32_t)total;
+  __syncthreads();
+  if (!over)
+    for (int m = t; m < (int)total; m += PLAN_THREADS) {
+      const int r = owner(s_put, p.n_req, m);
+      const int32_t page = p.tables[r * p.stride + m - s_put[r]];
+      if (page >= p.n_pages) s_bad = 1;
+    }
+  __syncthreads();
+  if (over || s_bad) {                // more pages than there are: nothing is released
+    if (t == 0 && p.status) atomicOr(p.status, HC_ERR_RANGE);
+    return;
+  }
+  for (int m = t; m < (int)total; m += PLAN_THREADS) {
+    const int r = owner(s_put, p.n_req, m);
+    int32_t* at = p.tables + r * p.stride + m - s_put[r];
+    p.free_pages[n_free + m] = *at;
+    *at = -1;
+  }
+  if (t == 0) *p.n_free = n_free + (int)total;
+}
+
+// ---------------------------------------------------------------------------
+// rotary positions
+// ---------------------------------------------------------------------------
+template <typename T>
+struct Num;
+template <>
+struct Num<__half> {
+  static __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
+  static __device__ __forceinline__ __half from_f(float x) { return __float2half_rn(x); }
+};
+template <>
+struct Num<__nv_bfloat16> {
+  static __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+  static __device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __float2bfloat16_rn(x); }
+};
+
+// one output of a pair: x c + y s.  Queries in fp32 (one fma).  Keys in 64
+// bits, where both products are exact, then rounded to fp32 and to T: the
+// 16-bit value decides the byte that the cache holds, which then depends on no
+// order of operations.
+template <typename T, bool KEY>
+__device__ __forceinline__ T turn(T x, T y, float c, float s) {
+  if constexpr (KEY)
+    return Num<T>::from_f((float)fma((double)Num<T>::to_f(y), (double)s, (double)Num<T>::to_f(x) * (double)c));
+  else
+    return Num<T>::from_f(fmaf(Num<T>::to_f(y), s, Num<T>::to_f(x) * c));
+}
+
+struct RopeArgs {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  int64_t q_row, q_head, k_row, k_head, qo_row, qo_head, ko_row, ko_head;
+  const float* cos_t;
+  const float* sin_t;
+  int64_t table_rows;
+  const int64_t* positions;
+  int n_rows, nq, nk, dim, rot;       // nk: key heads rotated by rope_rows (0 where they go into the cache)
+  int interleaved;
+  int slots;                          // heads of one row worked on at once
+  int32_t* status;
+};
+
+// position of a row: -1 for a row to leave alone (padding, or outside the tables)
+__device__ __forceinline__ int64_t checked_pos(const int64_t* positions, int row, int64_t table_rows,
+                                               int32_t* status) {
+  const int64_t pos = positions[row];
+  if (pos >= -1 && pos < table_rows) return pos;
+  if (status) atomicOr(status, HC_ERR_RANGE);
+  return -1;
+}
+
+// Vector form: a unit is 8 pairs (two 16-byte pieces of a head) or 16
+// elements that pass through.  A thread keeps its unit's 8 angles and walks
+// the row's heads with stride `slots`.  HBM-bound: each element read and
+// written once.
+template <typename T, bool KEY>
+__device__ __forceinline__ void rope_unit(const T* src, T* dst, int a0, int b0, bool turned, bool interleaved,
+                                          const float (&c)[8], const float (&s)[8]) {
+  __align__(16) T a[8], b[8], x[8], y[8];
+  *reinterpret_cast<uint4*>(a) = *reinterpret_cast<const uint4*>(src + a0);
+  *reinterpret_cast<uint4*>(b) = *reinterpret_cast<const uint4*>(src + b0);
+  if (!turned) {
+    *reinterpret_cast<uint4*>(dst + a0) = *reinterpret_cast<const uint4*>(a);
+    *reinterpret_cast<uint4*>(dst + b0) = *reinterpret_cast<const uint4*>(b);
+    return;
+  }
+  if (interleaved) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = turn<T, KEY>(a[2 * i], a[2 * i + 1], c[i], -s[i]);
+      x[2 * i + 1] = turn<T, KEY>(a[2 * i + 1], a[2 * i], c[i], s[i]);
+      y[2 * i] = turn<T, KEY>(b[2 * i], b[2 * i + 1], c[4 + i], -s[4 + i]);
+      y[2 * i + 1] = turn<T, KEY>(b[2 * i + 1], b[2 * i], c[4 + i], s[4 + i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[i] = turn<T, KEY>(a[i], b[i], c[i], -s[i]);
+      y[i] = turn<T, KEY>(b[i], a[i], c[i], s[i]);
+    }
+  }
+  *reinterpret_cast<uint4*>(dst + a0) = *reinterpret_cast<const uint4*>(x);
+  *reinterpret_cast<uint4*>(dst + b0) = *reinterpret_cast<const uint4*>(y);
+}
+
+template <typename T>
+__device__ __forceinline__ void rope_rows_vec(const RopeArgs& p, int64_t item0, int64_t items) {
+  const int units = p.dim / 16, heads = p.nq + p.nk;
+  const int64_t total = (int64_t)p.n_rows * p.slots * units;
+  for (int64_t it = item0; it < total; it += items) {
+    const int u = (int)(it % units), slot = (int)((it / units) % p.slots), row = (int)(it / units / p.slots);
+    const int64_t pos = checked_pos(p.positions, row, p.table_rows, p.status);
+    if (pos < 0) continue;
+    const bool turned = u < p.rot / 16;
+    float c[8], s[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = s[i] = 0.0f;
+    if (turned) {
+      const float4* cr = reinterpret_cast<const float4*>(p.cos_t + pos * (p.rot / 2) + 8 * u);
+      const float4* sr = reinterpret_cast<const float4*>(p.sin_t + pos * (p.rot / 2) + 8 * u);
+      *reinterpret_cast<float4*>(c) = __ldg(cr);
+      *reinterpret_cast<float4*>(c + 4) = __ldg(cr + 1);
+      *reinterpret_cast<float4*>(s) = __ldg(sr);
+      *reinterpret_cast<float4*>(s + 4) = __ldg(sr + 1);
+    }
+    const bool pairs = p.interleaved || !turned;
+    const int a0 = pairs ? 16 * u : 8 * u, b0 = pairs ? 16 * u + 8 : p.rot / 2 + 8 * u;
+    for (int h = slot; h < heads; h += p.slots) {
+      if (h < p.nq) {
+        const T* src = static_cast<const T*>(p.q) + row * p.q_row + h * p.q_head;
+        T* dst = static_cast<T*>(p.q_out) + row * p.qo_row + h * p.qo_head;
+        if (turned || src != dst) rope_unit<T, false>(src, dst, a0, b0, turned, p.interleaved, c, s);
+      } else {
+        const T* src = static_cast<const T*>(p.k) + row * p.k_row + (h - p.nq) * p.k_head;
+        T* dst = static_cast<T*>(p.k_out) + row * p.ko_row + (h - p.nq) * p.ko_head;
+        if (turned || src != dst) rope_unit<T, true>(src, dst, a0, b0, turned, p.interleaved, c, s);
+      }
+    }
+  }
+}
+
+// Any rotary size, stride and alignment: a thread per pair or passing element.
+template <typename T>
+__device__ __forceinline__ void rope_rows_any(const RopeArgs& p, int64_t item0, int64_t items) {
+  const int half = p.rot / 2, units = half + p.dim - p.rot, heads = p.nq + p.nk;
+  const int64_t total = (int64_t)p.n_rows * heads * units;
+  for (int64_t it = item0; it < total; it += items) {
+    const int u = (int)(it % units), h = (int)((it / units) % heads), row = (int)(it / units / heads);
+    const int64_t pos = checked_pos(p.positions, row, p.table_rows, p.status);
+    if (pos < 0) continue;
+    const bool key = h >= p.nq;
+    const T* src = key ? static_cast<const T*>(p.k) + row * p.k_row + (h - p.nq) * p.k_head
+                       : static_cast<const T*>(p.q) + row * p.q_row + h * p.q_head;
+    T* dst = key ? static_cast<T*>(p.k_out) + row * p.ko_row + (h - p.nq) * p.ko_head
+                 : static_cast<T*>(p.q_out) + row * p.qo_row + h * p.qo_head;
+    if (u >= half) {
+      dst[half + u] = src[half + u];
+      continue;
+    }
+    const int i = p.interleaved ? 2 * u : u, j = p.interleaved ? 2 * u + 1 : u + half;
+    const float c = __ldg(p.cos_t + pos * half + u), s = __ldg(p.sin_t + pos * half + u);
+    const T a = src[i], b = src[j];
+    dst[i] = key ? turn<T, true>(a, b, c, -s) : turn<T, false>(a, b, c, -s);
+    dst[j] = key ? turn<T, true>(b, a, c, s) : turn<T, false>(b, a, c, s);
+  }
+}
+
+constexpr int ROPE_THREADS = 256;
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const RopeArgs p) {
+  const int64_t item0 = (int64_t)blockIdx.x * ROPE_THREADS + threadIdx.x, items = (int64_t)gridDim.x * ROPE_THREADS;
+  if constexpr (VEC) rope_rows_vec<T>(p, item0, items);
+  else rope_rows_any<T>(p, item0, items);
+}
+
+// ---------------------------------------------------------------------------
+// the write of a step's keys and values
+// ---------------------------------------------------------------------------
+constexpr int E_MIN = -40, E_MAX = 40;  // exponents of a page scale
+constexpr int CHUNK = 16;               // rows a warp holds at once
+constexpr int APPEND_THREADS = 256;
+constexpr int APPEND_WARPS = APPEND_THREADS / 32;
+
+struct AppendArgs {
+  uint8_t* pages[2];                  // keys, values
+  float* scales[2];
+  int n_pages, n_kv, page_size, page_log2;
+  const void* src[2];
+  int64_t src_row[2], src_head[2];
+  const int64_t* slots;
+  int n_rows;
+  int seg;                            // rows a CTA looks for runs in
+  // rotation of the keys (fused form)
+  const float* cos_t;
+  const float* sin_t;
+  int64_t table_rows;
+  const int64_t* positions;
+  int rot, interleaved;
+  int32_t* status;
+};
+
+// exponent e of the smallest power of two with x <= 448 * 2^e, x >= 0 finite
+__device__ __forceinline__ int scale_exponent(float x) {
+  const uint32_t b = __float_as_uint(x);
+  if (b < 0x00800000u) return E_MIN;                 // zero and subnormals
+  // x = m 2^k with m in [1, 2); 448 = 1.75 * 2^8
+  const int k = (int)(b >> 23) - 127;
+  const int e = k - 8 + ((b & 0x007fffffu) > 0x00600000u ? 1 : 0);
+  return max(E_MIN, min(E_MAX, e));
+}
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// e4m3 byte of x (finite, |x| at most 448 after saturation), round to nearest even
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  unsigned short r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// One warp writes one run (the consecutive rows that enter one page) of one
+// head's keys or values.  EL elements of a row per lane; the run's rows are
+// held 16 at a time, and read again when the run is longer (its largest
+// value has to be known first).  Latency-bound for decode (one row a run),
+// HBM-bound for prompts.
+template <typename T, int EL, bool VEC, bool ROPE>
+__device__ __forceinline__ void append_run(const AppendArgs& p, int which, int head, int row0, int n, int64_t slot0) {
+  constexpr int D = 32 * EL;
+  const int lane = threadIdx.x & 31;
+  const int64_t page = slot0 >> p.page_log2;
+  const int lo = (int)slot0 & (p.page_size - 1);
+  uint8_t* dst = p.pages[which] + (page * p.n_kv + head) * p.page_size * D;
+  float* scale_at = p.scales[which] + page * p.n_kv + head;
+  const T* src = static_cast<const T*>(p.src[which]) + head * p.src_head[which];
+  const int64_t step = p.src_row[which];
+  const float old = lo ? *scale_at : 0.0f;           // a run from the page's first row begins the page anew
+  const int d0 = EL * lane;
+
+  auto load = [&](int row, T (&x)[EL]) {
+    const T* at = src + row * step;
+    if constexpr (VEC) {
+      if constexpr (EL == 4) *reinterpret_cast<uint2*>(x) = __ldg(reinterpret_cast<const uint2*>(at + d0));
+      else *reinterpret_cast<uint32_t*>(x) = __ldg(reinterpret_cast<const uint32_t*>(at + d0));
+    } else {
+#pragma unroll
+      for (int e = 0; e < EL; ++e) x[e] = at[d0 + e];
+    }
+    if constexpr (ROPE) {
+      if (which == 0) {
+        const int64_t pos = p.positions[row];
+        const int half = p.rot / 2;
+        T y[EL];
+#pragma unroll
+        for (int e = 0; e < EL; ++e) {
+          const int d = d0 + e;
+          y[e] = x[e];
+          if (d >= p.rot) continue;
+          const bool second = p.interleaved ? (d & 1) : d >= half;
+          const int pair = p.interleaved ? d >> 1 : second ? d - half : d;
+          const T other = at[p.interleaved ? d ^ 1 : second ? d - half : d + half];
+          const float c = __ldg(p.cos_t + pos * half + pair), s = __ldg(p.sin_t + pos * half + pair);
+          y[e] = turn<T, true>(x[e], other, c, second ? s : -s);
+        }
+#pragma unroll
+        for (int e = 0; e < EL; ++e) x[e] = y[e];
+      }
+    }
+  };
+
+  // largest finite value of the run
+  T x[CHUNK][EL];
+  float top = 0.0f;
+  bool odd = false;
+  for (int j0 = 0; j0 < n; j0 += CHUNK) {
+#pragma unroll
+    for (int j = 0; j < CHUNK; ++j)
+      if (j0 + j < n) load(row0 + j0 + j, x[j]);
+#pragma unroll
+    for (int j = 0; j < CHUNK; ++j)
+      if (j0 + j < n) {
+#pragma unroll
+        for (int e = 0; e < EL; ++e) {
+          const float a = fabsf(Num<T>::to_f(x[j][e]));
+          if (a < INFINITY) top = fmaxf(top, a);
+          else odd = true;
+        }
+      }
+  }
+  if (__any_sync(0xffffffffu, odd) && lane == 0 && p.status) atomicOr(p.status, HC_ERR_RANGE);
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float need = pow2f(scale_exponent(top));
+  const bool grown = need > old;
+  const float now = grown ? need : old;
+  const float inv = 1.0f / now;                      // exact: a power of two
+
+  // the page's older rows at the larger scale
+  if (lo && grown) {
+    const float f = old * inv;
+    for (int i = lane; i < lo * D / 16; i += 32) {
+      uint4* at = reinterpret_cast<uint4*>(dst) + i;
+      uint4 w = *at;
+      uint32_t* ws = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t h0 = e4m3x2_to_f16x2(ws[k]), h1 = e4m3x2_to_f16x2(ws[k] >> 16);
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h0));
+        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+        ws[k] = e4m3x2(a.x * f, a.y * f) | (e4m3x2(b.x * f, b.y * f) << 16);
+      }
+      *at = w;
+    }
+  }
+  if (lane == 0 && (grown || !lo)) *scale_at = now;
+
+  for (int j0 = 0; j0 < n; j0 += CHUNK) {
+    if (n > CHUNK) {
+#pragma unroll
+      for (int j = 0; j < CHUNK; ++j)
+        if (j0 + j < n) load(row0 + j0 + j, x[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < CHUNK; ++j)
+      if (j0 + j < n) {
+        float f[EL];
+#pragma unroll
+        for (int e = 0; e < EL; ++e) {
+          const float a = Num<T>::to_f(x[j][e]);
+          f[e] = a != a ? 0.0f : a * inv;            // NaN is stored as 0; infinities saturate
+        }
+        uint8_t* at = dst + (int64_t)(lo + j0 + j) * D + d0;
+        if constexpr (EL == 4) *reinterpret_cast<uint32_t*>(at) = e4m3x2(f[0], f[1]) | (e4m3x2(f[2], f[3]) << 16);
+        else *reinterpret_cast<unsigned short*>(at) = (unsigned short)e4m3x2(f[0], f[1]);
+      }
+  }
+}
+
+// slot of row t; -1 for padding (negative slots, and in the fused form rows
+// without a position in the tables); an index past the cache is flagged
+template <bool ROPE>
+__device__ __forceinline__ int64_t checked_slot(const AppendArgs& p, int t, bool flag) {
+  const int64_t slot = p.slots[t];
+  if (slot < 0) return -1;
+  bool bad = slot >= (int64_t)p.n_pages * p.page_size;
+  if constexpr (ROPE) {
+    const int64_t pos = p.positions[t];
+    if (pos == -1) return -1;
+    bad = bad || pos < 0 || pos >= p.table_rows;
+  }
+  if (bad && flag && p.status) atomicOr(p.status, HC_ERR_RANGE);
+  return bad ? -1 : slot;
+}
+
+// Runs that begin among rows [t0, t1), t1 - t0 <= 32: a row begins one unless
+// the row before it lies in the same page.  Rows of a page that do not follow
+// one another are flagged and left out.
+template <typename T, int EL, bool VEC, bool ROPE>
+__device__ __forceinline__ void append_rows(const AppendArgs& p, int t0, int t1, int item) {
+  const int lane = threadIdx.x & 31, which = item & 1, head = item >> 1;
+  const int mine = t0 + lane;
+  int64_t slot = -1;
+  bool begins = false;
+  if (mine < t1) {
+    slot = checked_slot<ROPE>(p, mine, item == 0);
+    const int64_t before = mine ? checked_slot<ROPE>(p, mine - 1, false) : -1;
+    const bool same = slot >= 0 && before >= 0 && before >> p.page_log2 == slot >> p.page_log2;
+    begins = slot >= 0 && !same;
+    if (same && before + 1 != slot && item == 0 && p.status) atomicOr(p.status, HC_ERR_RANGE);
+  }
+  for (uint32_t todo = __ballot_sync(0xffffffffu, begins); todo; todo &= todo - 1) {
+    const int from = __ffs(todo) - 1, t = t0 + from;
+    const int64_t first = __shfl_sync(0xffffffffu, slot, from);
+    const int left = min(p.page_size - ((int)first & (p.page_size - 1)), p.n_rows - t);
+    int n = 0;
+    for (int base = 0; base < left; base += 32) {
+      const int j = base + lane;
+      const bool follows = j < left && checked_slot<ROPE>(p, t + j, false) == first + j;
+      const uint32_t ok = __ballot_sync(0xffffffffu, follows);
+      n += ok == 0xffffffffu ? 32 : __ffs(~ok) - 1;
+      if (ok != 0xffffffffu) break;
+    }
+    append_run<T, EL, VEC, ROPE>(p, which, head, t, n, first);
+  }
+}
+
+// Blocks below `n_append` write the cache, the others rotate the queries.
+template <typename T, int EL, bool VEC, bool ROPE>
+__global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendArgs p, const RopeArgs rope, int n_append,
+                                                                int groups) {
+  if ((int)blockIdx.x < n_append) {
+    const int item = (int)(blockIdx.x % groups) * APPEND_WARPS + (threadIdx.x >> 5);
+    const int t0 = (int)(blockIdx.x / groups) * p.seg;
+    if (item < 2 * p.n_kv) append_rows<T, EL, VEC, ROPE>(p, t0, min(p.n_rows, t0 + p.seg), item);
+    return;
+  }
+  if constexpr (ROPE) {
+    const int64_t item0 = (int64_t)(blockIdx.x - n_append) * APPEND_THREADS + threadIdx.x;
+    const int64_t items = (int64_t)(gridDim.x - n_append) * APPEND_THREADS;
+    if constexpr (VEC) rope_rows_vec<T>(rope, item0, items);
+    else rope_rows_any<T>(rope, item0, items);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+inline bool multiple(int64_t v, int64_t m) { return v % m == 0; }
+inline bool aligned(const void* ptr, uintptr_t a) { return (reinterpret_cast<uintptr_t>(ptr) & (a - 1)) == 0; }
+
+int check_rope(const hc_rope_args* a, bool to_cache) {
+  if (!a || !a->cos_t || !a->sin_t) return HC_ERR_ARG;
+  if (a->n_rows != 0 && (!a->q || !a->q_out || !a->k || (!to_cache && !a->k_out) || !a->positions))
+    return HC_ERR_ARG;
+  if (a->n_rows < 0 || a->n_q_heads <= 0 || a->n_kv_heads <= 0 || a->head_dim <= 0 || a->rotary_dim <= 0 ||
+      a->rotary_dim > a->head_dim || (a->rotary_dim & 1) || a->table_rows <= 0 ||
+      (a->dtype != HC_F16 && a->dtype != HC_BF16) || a->interleaved < 0 || a->interleaved > 1)
+    return HC_ERR_ARG;
+  if (!aligned(a->q, 2) || !aligned(a->k, 2) || !aligned(a->q_out, 2) || !aligned(a->k_out, 2) ||
+      !aligned(a->cos_t, 4) || !aligned(a->sin_t, 4) || !aligned(a->positions, 8))
+    return HC_ERR_ARG;
+  return HC_OK;
+}
+
+// The vector form wants 16-byte pieces throughout and whole units of 8 pairs.
+bool rope_vec(const hc_rope_args* a, bool keys) {
+  bool ok = multiple(a->rotary_dim, 16) && multiple(a->head_dim, 16) && aligned(a->q, 16) && aligned(a->q_out, 16) &&
+            multiple(a->q_row, 8) && multiple(a->q_head, 8) && multiple(a->q_out_row, 8) &&
+            multiple(a->q_out_head, 8) && aligned(a->cos_t, 16) && aligned(a->sin_t, 16);
+  if (keys)
+    ok = ok && aligned(a->k, 16) && aligned(a->k_out, 16) && multiple(a->k_row, 8) && multiple(a->k_head, 8) &&
+         multiple(a->k_out_row, 8) && multiple(a->k_out_head, 8);
+  return ok;
+}
+
+RopeArgs rope_args(const hc_rope_args* a, bool keys, int32_t* status) {
+  RopeArgs p;
+  p.q = a->q;
+  p.k = a->k;
+  p.q_out = a->q_out;
+  p.k_out = a->k_out;
+  p.q_row = a->q_row;
+  p.q_head = a->q_head;
+  p.k_row = a->k_row;
+  p.k_head = a->k_head;
+  p.qo_row = a->q_out_row;
+  p.qo_head = a->q_out_head;
+  p.ko_row = a->k_out_row;
+  p.ko_head = a->k_out_head;
+  p.cos_t = a->cos_t;
+  p.sin_t = a->sin_t;
+  p.table_rows = a->table_rows;
+  p.positions = a->positions;
+  p.n_rows = a->n_rows;
+  p.nq = a->n_q_heads;
+  p.nk = keys ? a->n_kv_heads : 0;
+  p.dim = a->head_dim;
+  p.rot = a->rotary_dim;
+  p.interleaved = a->interleaved;
+  p.slots = 1;
+  p.status = status;
+  return p;
+}
+
+// Blocks of the rotation; sets how many heads of a row are worked on at once:
+// all of them while rows are few, a fifth when they fill the GPU anyway.
+int rope_blocks(RopeArgs& p, bool vec) {
+  const int heads = p.nq + p.nk;
+  int64_t threads;
+  if (vec) {
+    const int units = p.dim / 16;
+    p.slots = (int64_t)p.n_rows * units * heads <= 148 * 2048 ? heads : (heads + 4) / 5;
+    threads = (int64_t)p.n_rows * units * p.slots;
+  } else {
+    threads = (int64_t)p.n_rows * heads * (p.dim - p.rot / 2);
+  }
+  return (int)min((threads + ROPE_THREADS - 1) / ROPE_THREADS, (int64_t)148 * 64);
+}
+
+int check_pages(const hc_kv_pages* c) {
+  if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) return HC_ERR_ARG;
+  if (c->n_pages <= 0 || c->n_kv_heads <= 0) return HC_ERR_ARG;
+  if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 4) || !aligned(c->v_scale, 4))
+    return HC_ERR_ARG;
+  if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128)
+    return HC_ERR_UNSUPPORTED;
+  if (c->head_dim != 64 && c->head_dim != 128) return HC_ERR_UNSUPPORTED;
+  return HC_OK;
+}
+
+template <typename T>
+int launch_append(AppendArgs& p, const hc_rope_args* rope, const hc_kv_pages* c, cudaStream_t stream) {
+  RopeArgs ra = {};
+  int extra = 0;
+  const int align = c->head_dim == 128 ? 4 : 2;      // elements a lane loads at once
+  bool vec = aligned(p.src[0], 2 * align) && aligned(p.src[1], 2 * align) && multiple(p.src_row[0], align) &&
+             multiple(p.src_row[1], align) && multiple(p.src_head[0], align) && multiple(p.src_head[1], align);
+  if (rope) {
+    vec = vec && rope_vec(rope, false);
+    ra = rope_args(rope, false, p.status);
+    extra = rope_blocks(ra, vec);
+  }
+  // rows a CTA searches: one while rows are few (decode: every row is a run), more for prompts
+  p.seg = max(1, min(32, p.n_rows / 256));
+  const int groups = (2 * p.n_kv + APPEND_WARPS - 1) / APPEND_WARPS;
+  const int64_t n_append = (int64_t)((p.n_rows + p.seg - 1) / p.seg) * groups;
+  if (n_append + extra > INT32_MAX) return HC_ERR_UNSUPPORTED;
+  const dim3 grid((unsigned)(n_append + extra));
+#define GO(EL, V, R) append_kernel<T, EL, V, R><<<grid, APPEND_THREADS, 0, stream>>>(p, ra, (int)n_append, groups)
+  if (c->head_dim == 128) {
+    if (rope) {
+      if (vec) GO(4, true, true);
+      else GO(4, false, true);
+    } else {
+      if (vec) GO(4, true, false);
+      else GO(4, false, false);
+    }
+  } else {
+    if (rope) {
+      if (vec) GO(2, true, true);
+      else GO(2, false, true);
+    } else {
+      if (vec) GO(2, true, false);
+      else GO(2, false, false);
+    }
+  }
+#undef GO
+  return cudaGetLastError() == cudaSuccess ? HC_OK : HC_ERR_CUDA;
+}
+
+AppendArgs append_args(const hc_kv_pages* c, const void* k, int64_t k_row, int64_t k_head, const void* v,
+                       int64_t v_row, int64_t v_head, const int64_t* slots, int32_t n_rows, int32_t* status) {
+  AppendArgs p = {};
+  p.pages[0] = c->k;
+  p.pages[1] = c->v;
+  p.scales[0] = c->k_scale;
+  p.scales[1] = c->v_scale;
+  p.n_pages = c->n_pages;
+  p.n_kv = c->n_kv_heads;
+  p.page_size = c->page_size;
+  p.page_log2 = c->page_size == 16 ? 4 : c->page_size == 32 ? 5 : c->page_size == 64 ? 6 : 7;
+  p.src[0] = k;
+  p.src[1] = v;
+  p.src_row[0] = k_row;
+  p.src_row[1] = v_row;
+  p.src_head[0] = k_head;
+  p.src_head[1] = v_head;
+  p.slots = slots;
+  p.n_rows = n_rows;
+  p.status = status;
+  return p;
+}
+
+}  // namespace hcp
+
+using namespace hcp;
+
+extern "C" int hc_page_plan(const int32_t* starts, const int32_t* q_lens, int32_t n_requests, int32_t* tables,
+                            int64_t table_stride, int32_t table_width, const int32_t* free_pages, int32_t n_pages,
+                            int32_t* n_free, int32_t page_size, int32_t n_rows, int32_t* cu_q, int32_t* kv_lens,
+                            int64_t* positions, int64_t* slots, int32_t* status, hc_stream_t stream) {
+  if (!starts || !q_lens || !tables || !free_pages || !n_free || !cu_q || !kv_lens) return HC_ERR_ARG;
+  if (n_rows < 0 || (n_rows && (!positions || !slots))) return HC_ERR_ARG;
+  if (n_requests <= 0 || table_width <= 0 || table_stride < table_width || n_pages <= 0 || page_size <= 0)
+    return HC_ERR_ARG;
+  if ((int64_t)table_width * page_size > INT32_MAX) return HC_ERR_ARG;
+  if (n_requests > MAX_REQ) return HC_ERR_UNSUPPORTED;
+  PlanArgs p = {starts, q_lens, n_requests, tables, table_stride, table_width, free_pages, n_pages, n_free,
+                page_size, n_rows, cu_q, kv_lens, positions, slots, status};
+  const int cl = n_rows > PLAN_THREADS ? PLAN_CL : 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(cl);
+  cfg.blockDim = dim3(PLAN_THREADS);
+  cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cl;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, page_plan_kernel, p) == cudaSuccess ? HC_OK : HC_ERR_CUDA;
+}
+
+extern "C" int hc_page_release(const uint8_t* done, int32_t n_requests, int32_t* tables, int64_t table_stride,
+                               int32_t table_width, int32_t* free_pages, int32_t n_pages, int32_t* n_free,
+                               int32_t* status, hc_stream_t stream) {
+  if (!done || !tables || !free_pages || !n_free) return HC_ERR_ARG;
+  if (n_requests <= 0 || table_width <= 0 || table_stride < table_width || n_pages <= 0) return HC_ERR_ARG;
+  if (n_requests > MAX_REQ) return HC_ERR_UNSUPPORTED;
+  ReleaseArgs p = {done, n_requests, tables, table_stride, table_width, free_pages, n_pages, n_free, status};
+  page_release_kernel<<<1, PLAN_THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(p);
+  return cudaGetLastError() == cudaSuccess ? HC_OK : HC_ERR_CUDA;
+}
+
+extern "C" int hc_rope(const hc_rope_args* a, int32_t* status, hc_stream_t stream) {
+  const int rc = check_rope(a, false);
+  if (rc != HC_OK) return rc;
+  if (a->n_rows == 0) return HC_OK;
+  const bool vec = rope_vec(a, true);
+  RopeArgs p = rope_args(a, true, status);
+  const int blocks = rope_blocks(p, vec);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (a->dtype == HC_F16) {
+    if (vec) rope_kernel<__half, true><<<blocks, ROPE_THREADS, 0, s>>>(p);
+    else rope_kernel<__half, false><<<blocks, ROPE_THREADS, 0, s>>>(p);
+  } else {
+    if (vec) rope_kernel<__nv_bfloat16, true><<<blocks, ROPE_THREADS, 0, s>>>(p);
+    else rope_kernel<__nv_bfloat16, false><<<blocks, ROPE_THREADS, 0, s>>>(p);
+  }
+  return cudaGetLastError() == cudaSuccess ? HC_OK : HC_ERR_CUDA;
+}
+
+extern "C" int hc_kv_append(const hc_kv_pages* cache, const void* k, int64_t k_row, int64_t k_head, const void* v,
+                            int64_t v_row, int64_t v_head, const int64_t* slots, int32_t n_rows, int32_t dtype,
+                            int32_t* status, hc_stream_t stream) {
+  if (n_rows < 0 || (n_rows && (!k || !v || !slots)) || (dtype != HC_F16 && dtype != HC_BF16)) return HC_ERR_ARG;
+  if (!aligned(k, 2) || !aligned(v, 2) || !aligned(slots, 8)) return HC_ERR_ARG;
+  const int rc = check_pages(cache);
+  if (rc != HC_OK) return rc;
+  if (n_rows == 0) return HC_OK;
+  AppendArgs p = append_args(cache, k, k_row, k_head, v, v_row, v_head, slots, n_rows, status);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return dtype == HC_F16 ? launch_append<__half>(p, nullptr, cache, s)
+                         : launch_append<__nv_bfloat16>(p, nullptr, cache, s);
+}
+
+extern "C" int hc_rope_append(const hc_rope_args* a, const hc_kv_pages* cache, const void* v, int64_t v_row,
+                              int64_t v_head, const int64_t* slots, int32_t* status, hc_stream_t stream) {
+  int rc = check_rope(a, true);
+  if (rc != HC_OK) return rc;
+  if ((a->n_rows && (!v || !slots)) || !aligned(v, 2) || !aligned(slots, 8)) return HC_ERR_ARG;
+  rc = check_pages(cache);
+  if (rc != HC_OK) return rc;
+  if (a->n_kv_heads != cache->n_kv_heads || a->head_dim != cache->head_dim) return HC_ERR_ARG;
+  if (a->n_rows == 0) return HC_OK;
+  AppendArgs p = append_args(cache, a->k, a->k_row, a->k_head, v, v_row, v_head, slots, a->n_rows, status);
+  p.cos_t = a->cos_t;
+  p.sin_t = a->sin_t;
+  p.table_rows = a->table_rows;
+  p.positions = a->positions;
+  p.rot = a->rotary_dim;
+  p.interleaved = a->interleaved;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return a->dtype == HC_F16 ? launch_append<__half>(p, a, cache, s) : launch_append<__nv_bfloat16>(p, a, cache, s);
+}

@@ -23,7 +23,7 @@ HC_ERR_UNSUPPORTED = 16
 
 HC_F32, HC_BF16, HC_F16 = 0, 1, 2
 HC_ACT_SILU, HC_ACT_RELU = 0, 1
-ABI_VERSION = 3
+ABI_VERSION = 4
 
 TABLE_SIZE = 65536
 
@@ -93,6 +93,14 @@ _SIGS = {
     "hc_attn_decode": (c_i32, [c_p, c_p, c_p, c_p, c_p, c_p, c_i32, c_i32, c_i32, c_i32, c_p, c_p, c_p]),
     "hc_xchg_buffer_bytes": (c_i64, [c_i32, c_i64]),
     "hc_xchg_sum": (c_i32, [c_p, c_i64, c_p, c_i64, c_p, c_p, c_p]),
+    "hc_page_plan": (c_i32, [c_p, c_p, c_i32, c_p, c_i64, c_i32, c_p, c_i32, c_p, c_i32, c_i32, c_p, c_p, c_p, c_p,
+                             c_p, c_p]),
+    "hc_page_release": (c_i32, [c_p, c_i32, c_p, c_i64, c_i32, c_p, c_i32, c_p, c_p, c_p]),
+    "hc_rope": (c_i32, [c_p, c_p, c_p]),
+    "hc_kv_append": (c_i32, [c_p, c_p, c_i64, c_i64, c_p, c_i64, c_i64, c_p, c_i32, c_i32, c_p, c_p]),
+    "hc_rope_append": (c_i32, [c_p, c_p, c_p, c_i64, c_i64, c_p, c_p, c_p]),
+    "hc_paged_attn_workspace_bytes": (c_i64, [c_i32, c_i32, c_i32, c_i32, c_i32]),
+    "hc_paged_attn": (c_i32, [c_p, c_p, c_p, c_i64, c_p, c_p]),
 }
 
 
@@ -102,6 +110,29 @@ class TPDesc(ctypes.Structure):
                 ("words_n", ctypes.c_int32), ("peer_buf", ctypes.c_void_p), ("seq_base", ctypes.c_uint32),
                 ("wait_ns", ctypes.c_uint64), ("predict_last", ctypes.c_int32),
                 ("io_f16", ctypes.c_int32)]
+
+
+class KVPages(ctypes.Structure):
+    """Mirror of hc_kv_pages (include/hotcold.h)."""
+    _fields_ = [("k", c_p), ("v", c_p), ("k_scale", c_p), ("v_scale", c_p), ("n_pages", c_i32),
+                ("n_kv_heads", c_i32), ("page_size", c_i32), ("head_dim", c_i32)]
+
+
+class RopeArgs(ctypes.Structure):
+    """Mirror of hc_rope_args (include/hotcold.h)."""
+    _fields_ = [("q", c_p), ("k", c_p), ("q_out", c_p), ("k_out", c_p), ("q_row", c_i64), ("q_head", c_i64),
+                ("k_row", c_i64), ("k_head", c_i64), ("q_out_row", c_i64), ("q_out_head", c_i64),
+                ("k_out_row", c_i64), ("k_out_head", c_i64), ("cos_t", c_p), ("sin_t", c_p), ("table_rows", c_i64),
+                ("positions", c_p), ("n_rows", c_i32), ("n_q_heads", c_i32), ("n_kv_heads", c_i32),
+                ("head_dim", c_i32), ("rotary_dim", c_i32), ("interleaved", c_i32), ("dtype", c_i32)]
+
+
+class AttnArgs(ctypes.Structure):
+    """Mirror of hc_attn_args (include/hotcold.h)."""
+    _fields_ = [("q", c_p), ("out", c_p), ("lse", c_p), ("q_row", c_i64), ("q_head", c_i64), ("out_row", c_i64),
+                ("out_head", c_i64), ("tables", c_p), ("table_stride", c_i64), ("table_width", c_i32),
+                ("cu_q", c_p), ("kv_lens", c_p), ("n_requests", c_i32), ("n_rows", c_i32), ("max_q", c_i32),
+                ("n_q_heads", c_i32), ("scale", c_f), ("dtype", c_i32)]
 
 
 def _load():

@@ -55,7 +55,7 @@ typedef struct CUstream_st* hc_stream_t; /* == cudaStream_t */
 #define HC_ACT_RELU 1
 
 /* Library identity / device checks.  hc_version returns HC_ABI_VERSION. */
-#define HC_ABI_VERSION 3
+#define HC_ABI_VERSION 4
 HC_API int hc_version(void);
 HC_API const char* hc_status_string(int status);
 /* Number of SMs of the current device, or -1 when no CUDA device is usable. */
@@ -532,6 +532,168 @@ HC_API int hc_fp8_gemv_ex(const uint8_t* w, const float* row_scale, int64_t rows
 HC_API int hc_attn_decode(const void* qkv, const float* cos_t, const float* sin_t, const int64_t* pos,
                           void* k_cache, void* v_cache, int32_t capacity, int32_t n_q_heads, int32_t n_kv_heads,
                           int32_t head_dim, void* out, int32_t* status, hc_stream_t stream);
+
+/* ======================================================================= */
+/* Paged 8-bit key / value cache: a serving step of many requests          */
+/* ======================================================================= */
+
+/*
+ * A step serves requests 0..n_requests-1 of new lengths q_lens behind starts
+ * cached tokens.  Its tokens are rows: request r owns rows cu_q[r]..cu_q[r+1]
+ * of every [rows][...] array, in position order; rows behind cu_q[n_requests]
+ * are padding (a captured step has a fixed number of rows) and are left as
+ * they were.  A request's token at position pos lies at slot
+ * tables[r][pos / page_size] * page_size + pos % page_size of the cache.
+ * The order of a layer is hc_page_plan (once per step), hc_rope_append,
+ * hc_paged_attn.  `status` may be NULL in all of them.
+ */
+
+/*
+ * One layer's cache (host struct of device pointers).  A value is its e4m3
+ * byte times the scale of its page and head.  page_size is 16, 32, 64 or 128
+ * and head_dim 64 or 128 (else HC_ERR_UNSUPPORTED); k and v are 16-byte
+ * aligned.
+ */
+typedef struct hc_kv_pages {
+  uint8_t* k;       /* [n_pages][n_kv_heads][page_size][head_dim] e4m3 */
+  uint8_t* v;
+  float* k_scale;   /* [n_pages][n_kv_heads] */
+  float* v_scale;
+  int32_t n_pages, n_kv_heads, page_size, head_dim;
+} hc_kv_pages;
+
+/*
+ * hc_page_plan -- block tables and slot maps of a step from its lengths.
+ *   starts, q_lens [n_requests] int32: tokens in the cache, new tokens (a
+ *              request that sits the step out has 0)
+ *   tables     [n_requests] rows of table_width page ids, table_stride apart;
+ *              an entry below 0 is missing, the entries in place are a prefix
+ *              of each row.  Missing pages of the new positions are popped
+ *              from the stack free_pages[0..*n_free), in request order and
+ *              then page order; pages already in place are kept, so the same
+ *              step planned again takes nothing
+ *   n_free     device int32, lowered by the pages taken
+ *   cu_q [n_requests + 1], kv_lens [n_requests] (starts + q_lens) int32;
+ *   positions, slots [n_rows] int64, -1 behind the last token
+ * When a length is negative or past the table, the rows do not hold the
+ * tokens or the pages run out: HC_ERR_RANGE, nothing is taken, cu_q is all 0,
+ * kv_lens = starts and every row is padding.  A table entry or free page
+ * outside [0, n_pages) sets HC_ERR_RANGE and gives its rows slot -1.
+ * n_requests <= 2048 (else HC_ERR_UNSUPPORTED).  One launch, no workspace.
+ */
+HC_API int hc_page_plan(const int32_t* starts, const int32_t* q_lens, int32_t n_requests, int32_t* tables,
+                        int64_t table_stride, int32_t table_width, const int32_t* free_pages, int32_t n_pages,
+                        int32_t* n_free, int32_t page_size, int32_t n_rows, int32_t* cu_q, int32_t* kv_lens,
+                        int64_t* positions, int64_t* slots, int32_t* status, hc_stream_t stream);
+
+/*
+ * hc_page_release -- the pages of every request with done[r] != 0 go back
+ * onto the stack and its table row becomes missing (-1).  More pages than
+ * n_pages in all, or an id outside [0, n_pages): HC_ERR_RANGE and nothing is
+ * released.  A page shared by two tables is not known here: release one.
+ */
+HC_API int hc_page_release(const uint8_t* done, int32_t n_requests, int32_t* tables, int64_t table_stride,
+                           int32_t table_width, int32_t* free_pages, int32_t n_pages, int32_t* n_free,
+                           int32_t* status, hc_stream_t stream);
+
+/*
+ * Arguments of the rotary entry points (host struct of device pointers).
+ * Rows and heads are strided (in elements; a head's elements are contiguous),
+ * so q, k and v may be views of one projection's rows.
+ */
+typedef struct hc_rope_args {
+  const void* q;
+  const void* k;
+  void* q_out;                      /* may be q */
+  void* k_out;                      /* may be k; not used by hc_rope_append */
+  int64_t q_row, q_head, k_row, k_head;
+  int64_t q_out_row, q_out_head, k_out_row, k_out_head;
+  const float* cos_t;               /* [table_rows][rotary_dim / 2] fp32 */
+  const float* sin_t;
+  int64_t table_rows;
+  const int64_t* positions;         /* [n_rows]; -1 = padding */
+  int32_t n_rows, n_q_heads, n_kv_heads, head_dim;
+  int32_t rotary_dim;               /* even, <= head_dim; the rest of a head passes through */
+  int32_t interleaved;              /* 0: pairs (i, i + rotary_dim / 2); 1: pairs (2i, 2i + 1) */
+  int32_t dtype;                    /* HC_F16 or HC_BF16 */
+} hc_rope_args;
+
+/*
+ * hc_rope -- rotary positions of q and k (the reference's apply_rotary_emb,
+ * engine.py:143-158, for any rows and layouts): each pair (a, b) becomes
+ * (a c - b s, a s + b c), rounded once.  A scaled context is in the tables.
+ * A position outside [-1, table_rows): HC_ERR_RANGE, its row is left alone.
+ */
+HC_API int hc_rope(const hc_rope_args* args, int32_t* status, hc_stream_t stream);
+
+/*
+ * hc_kv_append -- writes rows of keys and values ([n_rows] rows of n_kv_heads
+ * heads, strided as above) into their slots.  A slot below 0 is padding; one
+ * past the cache sets HC_ERR_RANGE and is skipped.  Slots of one call are
+ * distinct, and rows that enter one page follow one another in slot order
+ * (as hc_page_plan gives them); a row that does not follow its predecessor
+ * inside the same page sets HC_ERR_RANGE and is left out.
+ * The scale of a page and head is the smallest power of two 2^e, -40 <= e <=
+ * 40, with |x| <= 448 * 2^e for its finite values.  Rows that begin a page
+ * (its first slot among them) begin it anew; rows that enter it later raise
+ * the scale when they need to, and the rows before them are rounded again
+ * (which changes only values among e4m3's subnormals).  Infinities saturate
+ * at 448 times the scale, NaN becomes 0, and both set HC_ERR_RANGE: the cache
+ * never holds a NaN.
+ */
+HC_API int hc_kv_append(const hc_kv_pages* cache, const void* k, int64_t k_row, int64_t k_head, const void* v,
+                        int64_t v_row, int64_t v_head, const int64_t* slots, int32_t n_rows, int32_t dtype,
+                        int32_t* status, hc_stream_t stream);
+
+/*
+ * hc_rope_append -- hc_rope on q (into q_out) and on k, and hc_kv_append of
+ * the rotated k (rounded to dtype first) and of v, in one launch: the same
+ * bytes as the two calls.
+ */
+HC_API int hc_rope_append(const hc_rope_args* args, const hc_kv_pages* cache, const void* v, int64_t v_row,
+                          int64_t v_head, const int64_t* slots, int32_t* status, hc_stream_t stream);
+
+/*
+ * hc_paged_attn -- causal attention of a step's rows over the paged cache
+ * (the reference's LlamaAttention, engine.py:100-125, for many requests):
+ * the query of request r's token at position pos sees its positions 0..pos,
+ * pos counted so that its last row sits at kv_lens[r] - 1; query head h reads
+ * key-value head h / (n_q_heads / n_kv_heads).
+ *   q, out     [n_rows] rows of n_q_heads heads of head_dim (HC_F16 or
+ *              HC_BF16), strided in elements
+ *   lse        optional [n_rows][n_q_heads] fp32: log of the softmax's sum
+ *              (natural logarithm of sum exp(scale q k)); -inf for a row that
+ *              sees nothing, whose output is 0
+ *   tables, table_stride, table_width, cu_q, kv_lens  as in hc_page_plan
+ *   max_q      host: the largest q_lens (chooses the kernels; any value is
+ *              answered correctly)
+ *   workspace  hc_paged_attn_workspace_bytes(...) bytes, 16-byte aligned
+ *              (scratch; no initial contents needed; not shared by calls that
+ *              can overlap)
+ * Softmax statistics are fp32; a page id outside the cache, a length past the
+ * table or rows past n_rows set HC_ERR_RANGE and are left out.  Bytes of
+ * positions behind kv_lens are never used, whatever they hold.
+ * n_requests <= 2048, n_q_heads / n_kv_heads <= 16 (else HC_ERR_UNSUPPORTED).
+ */
+typedef struct hc_attn_args {
+  const void* q;
+  void* out;
+  float* lse;
+  int64_t q_row, q_head, out_row, out_head;
+  const int32_t* tables;
+  int64_t table_stride;
+  int32_t table_width;
+  const int32_t* cu_q;
+  const int32_t* kv_lens;
+  int32_t n_requests, n_rows, max_q, n_q_heads;
+  float scale;                      /* 1 / sqrt(head_dim) as a rule */
+  int32_t dtype;
+} hc_attn_args;
+
+HC_API int64_t hc_paged_attn_workspace_bytes(int32_t n_requests, int32_t n_rows, int32_t n_q_heads,
+                                             int32_t n_kv_heads, int32_t head_dim);
+HC_API int hc_paged_attn(const hc_attn_args* args, const hc_kv_pages* cache, void* workspace,
+                         int64_t workspace_bytes, int32_t* status, hc_stream_t stream);
 
 #ifdef __cplusplus
 }
