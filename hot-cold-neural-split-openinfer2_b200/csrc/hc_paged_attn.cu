@@ -17,79 +17,17 @@
 // value scale costs nothing and p (rounded to f16 for the product: relative
 // 2^-11, like the output) is as large as the running maximum allows.  m moves
 // only when a score passes it by 2^8, which f16 holds easily.
-#include <type_traits>
-
-#include "hc_common.cuh"
+#include "hc_paged_attn.cuh"
 
 namespace hca8 {
-using namespace hc;
 
-constexpr int MAX_REQ = 2048;
 constexpr int CHUNK = 16;              // keys per chunk; no page is smaller
 constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
 constexpr int STAGES = 4;              // chunks in flight per warp
+constexpr int SMALL = 16;              // rows of a request and head that these kernels take
 constexpr int MIN_SHARE = WARPS;       // chunks of a share at least: one per warp
-constexpr float M_NONE = -1e30f;       // reference before the first key
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr float LN2 = 0.6931471805599453f;
 
-struct AttnParams {
-  const void* q;
-  void* out;
-  float* lse;
-  int64_t q_row, q_head, o_row, o_head;
-  const int32_t* tables;
-  int64_t t_stride;
-  int width;
-  const int32_t* cu_q;
-  const int32_t* kv_lens;
-  int n_req, n_rows, nq, nkv, g;
-  float scale2;                        // scale * log2(e)
-  const uint8_t* kp;
-  const uint8_t* vp;
-  const float* ks;
-  const float* vs;
-  int n_pages, page_log2;
-  float* part;                         // [2 grid][RT (D + 2)]
-  int4* cuts;                          // [grid]
-  int32_t* status;
-};
-
-template <typename T>
-__device__ __forceinline__ float load_f(const T* p);
-template <>
-__device__ __forceinline__ float load_f(const __half* p) { return __half2float(*p); }
-template <>
-__device__ __forceinline__ float load_f(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <typename T>
-__device__ __forceinline__ float2 unpack2(uint32_t w);
-template <>
-__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
-  return __half22float2(*reinterpret_cast<const __half2*>(&w));
-}
-template <>
-__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
-  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -118,23 +56,6 @@ __device__ __forceinline__ uint2 lds64(uint32_t addr) {
   uint2 v;
   asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
   return v;
-}
-
-// new tokens and cached length of request r; q_len 0 when the step leaves it out
-struct Req {
-  int q0, q_len, kv;
-};
-__device__ __forceinline__ Req request(const AttnParams& p, int r, bool flag) {
-  Req x;
-  x.q0 = p.cu_q[r];
-  const int q1 = p.cu_q[r + 1];
-  x.kv = p.kv_lens[r];
-  x.q_len = q1 - x.q0;
-  if (x.q0 < 0 || q1 < x.q0 || q1 > p.n_rows || x.kv < 0 || x.kv > ((int64_t)p.width << p.page_log2)) {
-    if (flag && p.status) atomicOr(p.status, HC_ERR_RANGE);
-    x.q_len = 0;
-  }
-  return x;
 }
 
 // Byte offset of 16-byte piece x of key row `key` in a chunk of [16][D] bytes.
@@ -701,7 +622,17 @@ extern "C" int hc_paged_attn(const hc_attn_args* a, const hc_kv_pages* c, void* 
   p.page_log2 = c->page_size == 16 ? 4 : c->page_size == 32 ? 5 : c->page_size == 64 ? 6 : 7;
   p.status = status;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const int rows = (int)min((int64_t)a->max_q * p.g, (int64_t)64);
-  return a->dtype == HC_F16 ? launch_typed<__half>(p, c->head_dim, rows, workspace, s)
-                            : launch_typed<__nv_bfloat16>(p, c->head_dim, rows, workspace, s);
+  // Up to SMALL rows of a request and head the keys are split over the GPU; more fill the tensor cores' tiles.
+  const int64_t rows = (int64_t)a->max_q * p.g;
+  p.rows_from = 0;
+  p.rows_to = INT32_MAX;
+  if (rows > SMALL) {
+    p.rows_from = SMALL + 1;
+    const int rc = launch_prefill(p, a->dtype, c->head_dim, s);
+    if (rc != HC_OK) return rc;
+    p.rows_from = 0;
+    p.rows_to = SMALL + 1;
+  }
+  return a->dtype == HC_F16 ? launch_typed<__half>(p, c->head_dim, (int)min(rows, (int64_t)64), workspace, s)
+                            : launch_typed<__nv_bfloat16>(p, c->head_dim, (int)min(rows, (int64_t)64), workspace, s);
 }
