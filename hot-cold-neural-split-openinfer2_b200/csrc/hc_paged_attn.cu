@@ -22,11 +22,14 @@
 namespace hca8 {
 
 constexpr int CHUNK = 16;              // keys per chunk; no page is smaller
-constexpr int THREADS = 256;
+constexpr int THREADS = 128;
 constexpr int WARPS = THREADS / 32;
-constexpr int STAGES = 4;              // chunks in flight per warp
+constexpr int STAGES = 3;              // chunks in flight per warp
+constexpr int ITEM_COST = 16;          // what beginning an item costs, in chunks
+constexpr uint32_t NONE = 0xffffffffu;
+constexpr int KEPT_REQ = 256;          // requests whose lengths stay in shared memory
 constexpr int SMALL = 16;              // rows of a request and head that these kernels take
-constexpr int MIN_SHARE = WARPS;       // chunks of a share at least: one per warp
+constexpr int MIN_SHARE = 2 * WARPS;   // units of a share at least
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -73,21 +76,42 @@ struct Cfg {
   static constexpr int PART = RT * (D + 2);                    // floats of one partial
 };
 
+// four dims of one output row from its sums
+template <typename T>
+__device__ __forceinline__ void write_row(const AttnParams& p, int tok, int head, int d, float M, float L, float a0,
+                                          float a1, float a2, float a3) {
+  const float inv = L > 0.0f ? __frcp_rn(L) : L;                     // no key: 0, and NaN stays NaN
+  T* out = static_cast<T*>(p.out) + (int64_t)tok * p.o_row + head * p.o_head + d;
+  const uint32_t w0 = pack2<T>(a0 * inv, a1 * inv), w1 = pack2<T>(a2 * inv, a3 * inv);
+  if ((reinterpret_cast<uintptr_t>(out) & 7) == 0) {
+    *reinterpret_cast<uint2*>(out) = make_uint2(w0, w1);
+  } else {
+    const T* a = reinterpret_cast<const T*>(&w0);
+    const T* b = reinterpret_cast<const T*>(&w1);
+    out[0] = a[0];
+    out[1] = a[1];
+    out[2] = b[0];
+    out[3] = b[1];
+  }
+  if (p.lse && d == 0) p.lse[(int64_t)tok * p.nq + head] = L == 0.0f ? -INFINITY : (M + __log2f(L)) * LN2;
+}
+
 // MMA shapes: S^T[16 keys][8 rows] = K Q^T and O^T[16 dims][8 rows] += V^T P^T,
 // so 8 rows fill an MMA's N and keys or dims its M.  Both inner dimensions may
 // be permuted freely as long as the two operands agree: lane (i, c) = (lane / 4,
 // lane % 4) takes dims [D/4 c, D/4 (c + 1)) of keys i, i + 8 and dims [D/8 i,
 // D/8 (i + 1)) of values 2c, 2c + 1, 2c + 8, 2c + 9, each contiguous in a row.
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(THREADS, 1) paged_attn_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) paged_attn_kernel(const AttnParams p) {
   using C = Cfg<T, D, NT>;
   constexpr int RT = C::RT;
   constexpr int KS = D / 16;           // k steps of S, also m tiles of O
   constexpr int KW = D / 16;           // words of a key row per lane
   constexpr int VW = D / 32;           // words of a value row per lane
   extern __shared__ __align__(16) uint8_t ring[];
-  __shared__ int64_t s_pre[MAX_REQ + 1];
+  int64_t* s_pre = reinterpret_cast<int64_t*>(ring + C::RING);       // [n_req + 1]
   __shared__ int64_t s_wsum[WARPS];
+  __shared__ Req s_req[KEPT_REQ];
   __shared__ float s_m[WARPS][RT], s_l[WARPS][RT];
   const int t = threadIdx.x, lane = t & 31, w = t >> 5;
   const int i8 = lane >> 2, c4 = lane & 3;
@@ -100,8 +124,9 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_kernel(const AttnParams
     const int r = t * per + i;
     if (r >= p.n_req) break;
     const Req x = request(p, r, blockIdx.x == 0);
+    if (p.n_req <= KEPT_REQ) s_req[r] = x;
     const int64_t tiles = (x.q_len * p.g + RT - 1) / RT;
-    sum += tiles * p.nkv * max(1, (x.kv + CHUNK - 1) / CHUNK);
+    sum += tiles * p.nkv * (ITEM_COST + max(1, (x.kv + CHUNK - 1) / CHUNK));
     s_pre[r + 1] = sum;
   }
   int64_t inc = sum;
@@ -128,34 +153,91 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_kernel(const AttnParams
   const int parts = (int)max((int64_t)1, min((int64_t)gridDim.x, total / MIN_SHARE));
   const int cta = blockIdx.x;
   if (cta >= parts || total == 0) {
-    if (t == 0) p.cuts[cta] = make_int4(0, 0, 0, 0);
+    if (t == 0) p.cuts[2 * cta] = make_int4(0, 0, 0, 0);
     return;
   }
   const int64_t lo = (int64_t)((uint64_t)total * cta / parts), hi = (int64_t)((uint64_t)total * (cta + 1) / parts);
-  if (t == 0) p.cuts[cta] = make_int4(0, 0, 0, 0);
+  if (t == 0) p.cuts[2 * cta] = make_int4(0, 0, 0, 0);
 
   const uint32_t my_ring = smem_u32(ring) + w * (STAGES * CHUNK * D * 2);
   int64_t u = lo;
   while (u < hi) {
-    // the item that holds chunk u
+    // the item that holds unit u: ITEM_COST units, then its chunks
     int r = 0;
     for (int b = p.n_req; b - r > 1;) {
       const int mid = (r + b) / 2;
       if (s_pre[mid] <= u) r = mid;
       else b = mid;
     }
-    const Req x = request(p, r, false);
+    const Req x = p.n_req <= KEPT_REQ ? s_req[r] : request(p, r, false);
     const int n_chunks = max(1, (x.kv + CHUNK - 1) / CHUNK);
     const int rows = x.q_len * p.g, tiles = (rows + RT - 1) / RT;
     const uint64_t off = (uint64_t)(u - s_pre[r]);
-    const int item = (int)(off / (uint32_t)n_chunks), c0 = (int)(off - (uint64_t)item * (uint32_t)n_chunks);
-    const int c1 = (int)min((int64_t)n_chunks, c0 + (hi - u));
+    const uint32_t span = n_chunks + ITEM_COST;
+    const int item = (int)(off / span), pos = (int)(off - (uint64_t)item * span) - ITEM_COST;
+    const int c0 = max(0, pos), c1 = (int)min((int64_t)n_chunks, pos + (hi - u));
+    u += c1 - pos;
+    if (c1 <= c0) continue;            // the share ends before the item's first chunk
     const int h = item / tiles, row0 = (item % tiles) * RT;
     const int n_here = min(RT, rows - row0);
     // key index of the last key that the first and the last row see
     const int behind = x.kv - x.q_len;
     const int lim_lo = behind + row0 / p.g, lim_hi = behind + (row0 + n_here - 1) / p.g;
     const int c_end = min(c1, lim_hi < 0 ? 0 : lim_hi / CHUNK + 1);
+
+    // This warp's chunks: c0 + w + WARPS k, k < count.  Lane k % 32 holds chunk
+    // k's place in the pools (in chunks; NONE without a page), its key scale
+    // and the logarithm and reciprocal of its value scale; two sets, for the
+    // even and odd 32 chunks.  The first loads start before anything else.
+    const int count = c_end > c0 + w ? (c_end - c0 - w + WARPS - 1) / WARPS : 0;
+    uint32_t at_[2];
+    float sk[2], sl[2], si[2];
+    auto load_places = [&](int batch, int set) {
+      const int k = batch * 32 + lane;
+      uint32_t at = NONE;
+      if (k < count) {
+        const int key = (c0 + w + WARPS * k) * CHUNK;
+        const int page = __ldg(p.tables + (int64_t)r * p.t_stride + (key >> p.page_log2));
+        if (page < 0 || page >= p.n_pages) {
+          if (p.status) atomicOr(p.status, HC_ERR_RANGE);
+        } else {
+          at = (uint32_t)(((((int64_t)page * p.nkv + h) << p.page_log2) + (key & ((1 << p.page_log2) - 1))) / CHUNK);
+        }
+      }
+      if (set) at_[1] = at;
+      else at_[0] = at;
+    };
+    auto load_scales = [&](int set) {
+      const uint32_t at = set ? at_[1] : at_[0];
+      float a = 0.0f, b = 1.0f;
+      if (at != NONE) {
+        const uint32_t head = at >> (p.page_log2 - 4);           // page * nkv + h
+        a = __ldg(p.ks + head);
+        b = fmaxf(__ldg(p.vs + head), 1e-30f);
+      }
+      const float lb = __log2f(b), ib = __frcp_rn(b);
+      if (set) sk[1] = a, sl[1] = lb, si[1] = ib;
+      else sk[0] = a, sl[0] = lb, si[0] = ib;
+    };
+    auto issue = [&](int k) {
+      const uint32_t at = __shfl_sync(0xffffffffu, (k >> 5) & 1 ? at_[1] : at_[0], k & 31);
+      if (k < count && at != NONE) {
+        const uint32_t dst = my_ring + (k % STAGES) * (CHUNK * D * 2);
+        const uint8_t* ksrc = p.kp + (uint64_t)at * (CHUNK * D) + lane * 16;
+        const uint8_t* vsrc = p.vp + (uint64_t)at * (CHUNK * D) + lane * 16;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+          const int b = (j * 32 + lane) * 16;
+          const uint32_t s = piece_at<D>(b / D, (b % D) / 16);
+          cp16(dst + s, ksrc + j * 512);
+          cp16(dst + CHUNK * D + s, vsrc + j * 512);
+        }
+      }
+      cp_commit();
+    };
+    load_places(0, 0);
+#pragma unroll
+    for (int k = 0; k < STAGES - 1; ++k) issue(k);
 
     // this lane's part of its query row(s), in f16, and the rows' factors
     uint32_t qf[NT][KS][2];
@@ -228,61 +310,24 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_kernel(const AttnParams
         for (int e = 0; e < 4; ++e) o[nt][k][e] = 0.0f;
     }
 
-    // This warp's chunks: c0 + w + WARPS k, k < count.  Lane k % 32 holds the
-    // page and scales of chunk k; two sets, for the even and odd 32 chunks.
-    const int count = c_end > c0 + w ? (c_end - c0 - w + WARPS - 1) / WARPS : 0;
-    int pg[2];
-    float sk[2], sv[2];
-    auto load_meta = [&](int batch, int set) {
-      const int k = batch * 32 + lane;
-      int page = -1;
-      if (k < count) {
-        page = __ldg(p.tables + (int64_t)r * p.t_stride + (((c0 + w + WARPS * k) * CHUNK) >> p.page_log2));
-        if (page < 0 || page >= p.n_pages) {
-          if (p.status) atomicOr(p.status, HC_ERR_RANGE);
-          page = -1;
-        }
-      }
-      float a = 0.0f, b = 1.0f;
-      if (page >= 0) {
-        a = __ldg(p.ks + (int64_t)page * p.nkv + h);
-        b = __ldg(p.vs + (int64_t)page * p.nkv + h);
-      }
-      if (set) pg[1] = page, sk[1] = a, sv[1] = b;
-      else pg[0] = page, sk[0] = a, sv[0] = b;
-    };
-    load_meta(0, 0);
-    load_meta(1, 1);
-    auto issue = [&](int k) {
-      const int page = __shfl_sync(0xffffffffu, (k >> 5) & 1 ? pg[1] : pg[0], k & 31);
-      if (k < count && page >= 0) {
-        const int key = (c0 + w + WARPS * k) * CHUNK;
-        const int64_t at = ((((int64_t)page * p.nkv + h) << p.page_log2) + (key & ((1 << p.page_log2) - 1))) * D;
-        const uint32_t dst = my_ring + (k % STAGES) * (CHUNK * D * 2);
-#pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
-          const int b = (j * 32 + lane) * 16;
-          const uint32_t s = piece_at<D>(b / D, (b % D) / 16);
-          cp16(dst + s, p.kp + at + b);
-          cp16(dst + CHUNK * D + s, p.vp + at + b);
-        }
-      }
-      cp_commit();
-    };
-#pragma unroll
-    for (int k = 0; k < STAGES - 1; ++k) issue(k);
-
+    load_places(1, 1);
+    load_scales(0);
+    load_scales(1);
     for (int k = 0; k < count; ++k) {
       cp_wait<STAGES - 2>();
       __syncwarp();
       issue(k + STAGES - 1);
       const int set = (k >> 5) & 1;
-      const int page = __shfl_sync(0xffffffffu, set ? pg[1] : pg[0], k & 31);
+      const uint32_t at = __shfl_sync(0xffffffffu, set ? at_[1] : at_[0], k & 31);
       const float kscale = __shfl_sync(0xffffffffu, set ? sk[1] : sk[0], k & 31);
-      const float vscale = fmaxf(__shfl_sync(0xffffffffu, set ? sv[1] : sv[0], k & 31), 1e-30f);
+      const float lv = __shfl_sync(0xffffffffu, set ? sl[1] : sl[0], k & 31);
+      const float iv = __shfl_sync(0xffffffffu, set ? si[1] : si[0], k & 31);
       const int key0 = (c0 + w + WARPS * k) * CHUNK;
-      if ((k & 31) == 31) load_meta((k >> 5) + 2, set);
-      if (page < 0) continue;
+      if ((k & 31) == 31) {
+        load_places((k >> 5) + 2, set);
+        load_scales(set);
+      }
+      if (at == NONE) continue;
       const uint32_t kb = my_ring + (k % STAGES) * (CHUNK * D * 2), vb = kb + CHUNK * D;
 
       // S^T
@@ -312,8 +357,6 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_kernel(const AttnParams
       }
 
       // weights
-      const float lv = __log2f(vscale);
-      const float iv = __frcp_rn(vscale);
       const bool masked = key0 + CHUNK - 1 > lim_lo;
       bool over = false;
 #pragma unroll
@@ -437,23 +480,8 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_kernel(const AttnParams
         a3 = fmaf(v.w, f, a3);
       }
       if (whole) {
-        if (row < n_here) {
-          const int tok = x.q0 + (row0 + row) / p.g, head = h * p.g + (row0 + row) % p.g;
-          const float inv = L > 0.0f ? __frcp_rn(L) : L;      // no key: 0, and NaN stays NaN
-          T* out = static_cast<T*>(p.out) + (int64_t)tok * p.o_row + head * p.o_head + d;
-          const uint32_t w0 = pack2<T>(a0 * inv, a1 * inv), w1 = pack2<T>(a2 * inv, a3 * inv);
-          if ((reinterpret_cast<uintptr_t>(out) & 7) == 0) {
-            *reinterpret_cast<uint2*>(out) = make_uint2(w0, w1);
-          } else {
-            const T* a = reinterpret_cast<const T*>(&w0);
-            const T* b = reinterpret_cast<const T*>(&w1);
-            out[0] = a[0];
-            out[1] = a[1];
-            out[2] = b[0];
-            out[3] = b[1];
-          }
-          if (p.lse && d == 0) p.lse[(int64_t)tok * p.nq + head] = L == 0.0f ? -INFINITY : (M + __log2f(L)) * LN2;
-        }
+        if (row < n_here)
+          write_row<T>(p, x.q0 + (row0 + row) / p.g, h * p.g + (row0 + row) % p.g, d, M, L, a0, a1, a2, a3);
       } else {
         *reinterpret_cast<float4*>(part + row * D + d) = make_float4(a0, a1, a2, a3);
         if (d == 0) {
@@ -464,60 +492,74 @@ __global__ void __launch_bounds__(THREADS, 1) paged_attn_kernel(const AttnParams
     }
     if (!whole && c0 == 0 && t == 0) {
       // the item's first piece: the pieces of CTAs cta .. last belong to it
-      const int last = (int)(((uint64_t)(u + n_chunks) * parts - 1) / (uint64_t)total);
-      p.cuts[cta] = make_int4(r, h, row0, last - cta + 1);
+      const int last = (int)(((uint64_t)(u + n_chunks - c1) * parts - 1) / (uint64_t)total);
+      p.cuts[2 * cta] = make_int4(r, h, row0, last - cta + 1);
+      p.cuts[2 * cta + 1] = make_int4(n_here, x.q0, 0, 0);
     }
     __syncthreads();
-    u += c1 - c0;
   }
 }
 
 // Joins the pieces of the items that the shares' borders divide, in the order
-// of the shares.
+// of the shares: two rows a CTA, 32 lanes of four dims each, the pieces dealt
+// to groups of lanes whose sums meet in shared memory.
+constexpr int JOIN_ROWS = 2;
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(THREADS) paged_join_kernel(const AttnParams p) {
   using C = Cfg<T, D, NT>;
   constexpr int RT = C::RT;
+  constexpr int LANES = D / 4, GROUPS = THREADS / (LANES * JOIN_ROWS);
+  __shared__ float s_acc[GROUPS][JOIN_ROWS][LANES][6];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int cta = blockIdx.x;
-  const int4 cut = p.cuts[cta];
-  if (cut.w == 0) return;
-  const Req x = request(p, cut.x, false);
-  const int h = cut.y, row0 = cut.z, n = cut.w;
-  const int n_here = min(RT, x.q_len * p.g - row0);
-  for (int e = threadIdx.x; e < n_here * D / 4; e += THREADS) {
-    const int row = e / (D / 4), d = (e % (D / 4)) * 4;
-    auto piece = [&](int k) { return p.part + (int64_t)(2 * (cta + k) + (k == 0 ? 1 : 0)) * C::PART; };
-    float M = M_NONE;
-    for (int k = 0; k < n; ++k) M = fmaxf(M, piece(k)[RT * D + row]);
-    float L = 0.0f, a0 = 0.0f, a1 = 0.0f, a2 = 0.0f, a3 = 0.0f;
-#pragma unroll 4
-    for (int k = 0; k < n; ++k) {
-      const float* q = piece(k);
-      const float f = ex2(q[RT * D + row] - M);
-      const float4 v = *reinterpret_cast<const float4*>(q + row * D + d);
-      L = fmaf(q[RT * D + RT + row], f, L);
-      a0 = fmaf(v.x, f, a0);
-      a1 = fmaf(v.y, f, a1);
-      a2 = fmaf(v.z, f, a2);
-      a3 = fmaf(v.w, f, a3);
+  const int4 cut = p.cuts[2 * cta], rest = p.cuts[2 * cta + 1];      // request, head, first row, pieces; rows, first token
+  const int n = cut.w;
+  const int row = blockIdx.y * JOIN_ROWS + (threadIdx.x / LANES) % JOIN_ROWS, d = (threadIdx.x % LANES) * 4;
+  if (n == 0 || blockIdx.y * JOIN_ROWS >= rest.x) return;
+  const int grp = threadIdx.x / (LANES * JOIN_ROWS);
+  // piece 0 is the last of its share (slot 1), the others are the first of theirs
+  const float* first = p.part + (int64_t)(2 * cta + 1) * C::PART;
+  const float* others = p.part + (int64_t)(2 * cta) * C::PART;
+  // running maximum, four pieces' loads at a time
+  float M = M_NONE, L = 0.0f, a0 = 0.0f, a1 = 0.0f, a2 = 0.0f, a3 = 0.0f;
+  for (int k0 = grp; k0 < n; k0 += 4 * GROUPS) {
+    float pm[4], pl[4];
+    float4 v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int k = k0 + e * GROUPS;
+      const float* q = k ? others + (int64_t)k * 2 * C::PART : first;
+      pm[e] = M_NONE, pl[e] = 0.0f, v[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (k < n) {
+        pm[e] = q[RT * D + row];
+        pl[e] = q[RT * D + RT + row];
+        v[e] = *reinterpret_cast<const float4*>(q + row * D + d);
+      }
     }
-    const int tok = x.q0 + (row0 + row) / p.g, head = h * p.g + (row0 + row) % p.g;
-    const float inv = L > 0.0f ? __frcp_rn(L) : L;
-    T* out = static_cast<T*>(p.out) + (int64_t)tok * p.o_row + head * p.o_head + d;
-    const uint32_t w0 = pack2<T>(a0 * inv, a1 * inv), w1 = pack2<T>(a2 * inv, a3 * inv);
-    if ((reinterpret_cast<uintptr_t>(out) & 7) == 0) {
-      *reinterpret_cast<uint2*>(out) = make_uint2(w0, w1);
-    } else {
-      const T* a = reinterpret_cast<const T*>(&w0);
-      const T* b = reinterpret_cast<const T*>(&w1);
-      out[0] = a[0];
-      out[1] = a[1];
-      out[2] = b[0];
-      out[3] = b[1];
+    const float M1 = fmaxf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), M), keep = ex2(M - M1);
+    M = M1, L *= keep, a0 *= keep, a1 *= keep, a2 *= keep, a3 *= keep;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float f = ex2(pm[e] - M);
+      L = fmaf(pl[e], f, L);
+      a0 = fmaf(v[e].x, f, a0);
+      a1 = fmaf(v[e].y, f, a1);
+      a2 = fmaf(v[e].z, f, a2);
+      a3 = fmaf(v[e].w, f, a3);
     }
-    if (p.lse && d == 0) p.lse[(int64_t)tok * p.nq + head] = L == 0.0f ? -INFINITY : (M + __log2f(L)) * LN2;
   }
+  float* mine = s_acc[grp][(threadIdx.x / LANES) % JOIN_ROWS][threadIdx.x % LANES];
+  mine[0] = L, mine[1] = a0, mine[2] = a1, mine[3] = a2, mine[4] = a3, mine[5] = M;
+  __syncthreads();
+  if (grp != 0 || row >= rest.x) return;
+#pragma unroll
+  for (int k = 1; k < GROUPS; ++k) {
+    const float* o = s_acc[k][(threadIdx.x / LANES) % JOIN_ROWS][threadIdx.x % LANES];
+    const float M1 = fmaxf(M, o[5]), f = ex2(M - M1), g = ex2(o[5] - M1);
+    M = M1, L = L * f + o[0] * g, a0 = a0 * f + o[1] * g, a1 = a1 * f + o[2] * g, a2 = a2 * f + o[3] * g;
+    a3 = a3 * f + o[4] * g;
+  }
+  write_row<T>(p, rest.y + (cut.z + row) / p.g, cut.y * p.g + (cut.z + row) % p.g, d, M, L, a0, a1, a2, a3);
 }
 
 int sm_count() {
@@ -527,24 +569,25 @@ int sm_count() {
     return 0;
   return n;
 }
-constexpr int MAX_GRID = 256;          // workspace sizing; a B200 has 148 SMs
+constexpr int MAX_GRID = 444;          // workspace sizing: 3 CTAs on each of a B200's 148 SMs
 
-int64_t workspace_need(int head_dim) { return MAX_GRID * 16ll + 2ll * MAX_GRID * 16 * (head_dim + 2) * 4; }
+int64_t workspace_need(int head_dim) { return MAX_GRID * 32ll + 2ll * MAX_GRID * 16 * (head_dim + 2) * 4; }
 
 template <typename T, int D, int NT>
 int launch(AttnParams& p, void* workspace, cudaStream_t stream) {
   using C = Cfg<T, D, NT>;
-  const int grid = min(sm_count(), MAX_GRID);
+  const int grid = min(sm_count() * (NT == 1 ? 3 : 2), MAX_GRID);      // resident CTAs: registers bound them
   if (grid <= 0) return HC_ERR_CUDA;
   p.cuts = static_cast<int4*>(workspace);
-  p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + MAX_GRID * 16);
-  if (cudaFuncSetAttribute(paged_attn_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::RING) !=
+  p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + MAX_GRID * 32);
+  const int smem = C::RING + (p.n_req + 1) * 8;
+  if (cudaFuncSetAttribute(paged_attn_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
       cudaSuccess)
     return HC_ERR_CUDA;
-  paged_attn_kernel<T, D, NT><<<grid, THREADS, C::RING, stream>>>(p);
+  paged_attn_kernel<T, D, NT><<<grid, THREADS, smem, stream>>>(p);
   if (cudaGetLastError() != cudaSuccess) return HC_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
+  cfg.gridDim = dim3(grid, C::RT / JOIN_ROWS);
   cfg.blockDim = dim3(THREADS);
   cfg.stream = stream;
   cudaLaunchAttribute at[1];

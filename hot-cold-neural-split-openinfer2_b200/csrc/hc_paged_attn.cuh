@@ -31,8 +31,8 @@ struct AttnParams {
   const float* vs;
   int n_pages, page_log2;
   int rows_from, rows_to;              // requests of rows_from <= q_len * g < rows_to are served
-  float* part;                         // [2 grid][RT (D + 2)]
-  int4* cuts;                          // [grid]
+  float* part;                         // [grid][2][RT (D + 2)]: partials of a share's first and last item
+  int4* cuts;                          // [grid][2]: the divided item that begins in a share
   int32_t* status;
 };
 
