@@ -26,8 +26,6 @@ constexpr int THREADS = 128;
 constexpr int WARPS = THREADS / 32;
 constexpr int STAGES = 3;              // chunks in flight per warp
 constexpr int ITEM_COST = 16;          // what beginning an item costs, in chunks
-constexpr uint32_t NONE = 0xffffffffu;
-constexpr int KEPT_REQ = 256;          // requests whose lengths stay in shared memory
 constexpr int SMALL = 16;              // rows of a request and head that these kernels take
 constexpr int MIN_SHARE = 2 * WARPS;   // units of a share at least
 

@@ -9,6 +9,8 @@ namespace hca8 {
 using namespace hc;
 
 constexpr int MAX_REQ = 2048;
+constexpr uint32_t NONE = 0xffffffffu; // no page
+constexpr int KEPT_REQ = 256;          // requests whose lengths stay in shared memory
 constexpr float M_NONE = -1e30f;       // softmax reference before the first key
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;

@@ -1,33 +1,40 @@
 // Paged attention of many rows (prompts) on the tcgen05 tensor cores.
 //
 // One CTA takes 256 rows (token, query head) of one request and key-value
-// head, as two groups of 128, and walks the request's keys 128 at a time:
-//   S = Q K^T   128 x 128 per group, accumulated in TMEM
+// head, as two groups of 128, and walks the request's keys 64 at a time:
+//   S = Q K^T   128 x 64 per group, accumulated in TMEM, two buffers a group
 //   P = 2^(S - m), f16, written over S in TMEM by the group's four warps (a
 //       thread has a row, so its maximum and sum need no exchange)
 //   O += P V    accumulated in TMEM, A operand P from TMEM
-// e4m3 keys and values become f16 (exactly) in shared memory; four warps load
-// a tile's bytes into registers one tile ahead, convert, and store the operand
-// layout.  The groups alternate: while one group's softmax runs, the tensor
-// cores work on the other's two products, and each conversion serves 256 rows.
+// e4m3 keys and values become f16 (exactly) in shared memory, 128 keys a tile
+// and two tiles deep: four warps load a tile's bytes into registers, convert,
+// and store the operand layout; each conversion serves 256 rows.  With two
+// score buffers a group's softmax runs on without waiting for its products,
+// and the tensor cores always have the other group's to do.
 //
 // Page scales: a key's scale joins the factor of its 16 score columns, a
 // value's scale enters as log2 in the exponent (see hc_paged_attn.cu).
 //
 // Operand layouts (128-byte swizzle, 8-row atoms of 1024 bytes): Q and K are
 // K-major, rows of 64 f16 per 16 KB block; V has the same image, read MN-major
-// (dims contiguous).  TMEM: S of group x at column 128 x (P over its first 64
-// columns), O at 256 + 128 x.
+// (dims contiguous).  TMEM: S of group x and buffer b at column 128 x + 64 b (P
+// over its first 32 columns), O at 256 + 128 x.  Each group's products are
+// issued by a thread of its own (one thread spent 2000 cycles on the 24 MMAs of
+// 64 keys, which take 1250) and run in the order it issues them, so a buffer is
+// written again without a wait for the product that read it.
 #include "hc_paged_attn.cuh"
 
 namespace hca8 {
 
-constexpr int PF_THREADS = 416;        // 8 softmax warps, 4 converter warps, 1 MMA warp
+constexpr int CONVERTERS = 4;          // warps
+constexpr int PF_THREADS = 256 + 32 * CONVERTERS + 64;      // 8 softmax warps, the converters, an MMA warp per group
+constexpr int MMA_WARP = 8 + CONVERTERS;
 constexpr int GROUP_ROWS = 128;
 constexpr int ROWS = 2 * GROUP_ROWS;
-constexpr int KT = 128;                // keys per tile
+constexpr int KT = 128;                // keys per converted tile
+constexpr int HALF = 64;               // keys per score buffer
 constexpr int SLICES = KT / 16;        // 16-key slices: no page is smaller
-constexpr uint64_t PF_WAIT_NS = 2000000000ull;
+constexpr uint32_t PF_TRIES = 1u << 22; // a wait gives up after so many tries (each suspends for a while)
 
 template <int D>
 struct Layout {
@@ -66,20 +73,40 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
                : "memory");
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+// generic stores to shared memory (this thread's, and others' it has synchronised with) before the tensor cores' reads
+__device__ __forceinline__ void fence_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
 #define R4(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3])
-// 32 columns of this thread's TMEM lane
+// 32 columns of this thread's TMEM lane; the values are there after tmem_wait_ld
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&v)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
       : R4(v, 0), R4(v, 4), R4(v, 8), R4(v, 12), R4(v, 16), R4(v, 20), R4(v, 24), R4(v, 28)
       : "r"(addr)
       : "memory");
 }
+// 16 columns, with the wait
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : R4(v, 0), R4(v, 4), R4(v, 8), R4(v, 12)
+      : "r"(addr)
+      : "memory");
+}
 #undef R4
+#define X4(v, i) "+r"(v[i]), "+r"(v[i + 1]), "+r"(v[i + 2]), "+r"(v[i + 3])
+// every load so far has arrived; v names the registers, so that nothing that reads them moves ahead of it
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : X4(v, 0), X4(v, 4), X4(v, 8), X4(v, 12), X4(v, 16), X4(v, 20), X4(v, 24), X4(v, 28)
+               :
+               : "memory");
+}
+#undef X4
 #define W4(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3])
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]) {
   asm volatile(
@@ -88,33 +115,118 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]
       W4(v, 0), W4(v, 4), W4(v, 8), W4(v, 12)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
-      W4(v, 0), W4(v, 4), W4(v, 8), W4(v, 12), W4(v, 16), W4(v, 20), W4(v, 24), W4(v, 28)
-      : "memory");
-}
 #undef W4
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void sts16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// two fp32 lanes in one instruction
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair2(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// Bounded wait, kept short: the roles' loops share the instruction caches.
+__device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity) {
+#pragma unroll 1
+  for (uint32_t n = 0; n < PF_TRIES; ++n)
+    if (mbar_try_wait(bar, parity)) return true;
+  return false;
+}
+
 struct Bars {
   uint64_t k_full[2], v_full[2];       // converters -> MMA
   uint64_t k_free[2], v_free[2];       // MMA -> converters
-  uint64_t s_full[2];                  // MMA -> group: S of the next tile (and every earlier product) is complete
-  uint64_t p_full[2];                  // group -> MMA: P is written
-  uint64_t done[2];                    // MMA -> group: all products complete
+  uint64_t s_full[2][2];               // MMA -> group: the buffer's scores are complete
+  uint64_t p_full[2][2];               // group -> MMA: the buffer's weights are written
+  uint64_t o_done[2];                  // MMA -> group: a half's product is in O
+  uint64_t done[2];                    // MMA -> group: all products are
   uint64_t meta[4];                    // converters -> groups: a tile's scales
-  uint64_t drain;
+  uint64_t drain[2];
 };
 
 // Shared by the roles of one CTA.
 struct Slice {
   float k, lv, iv;                     // key scale, log2 and reciprocal of the value scale
 };
+
+// factor of a slice's scores; never 0, which would make NaN of a masked score
+__device__ __forceinline__ float factor(float k, float fac) { return fmaxf(k * fac, 1e-37f); }
+// Columns past `last` are not seen.
+__device__ __forceinline__ void mask_row(uint32_t (&s)[2][32], int last) {
+#pragma unroll
+  for (int c = 0; c < HALF; ++c)
+    if (c > last) s[c >> 5][c & 31] = 0xff800000u;
+}
+// The largest exponent (base 2, scales applied) of this thread's row of a half.
+__device__ __forceinline__ float row_max(const uint32_t (&s)[2][32], const Slice* sl, float fac) {
+  float top = -INFINITY;
+#pragma unroll
+  for (int q = 0; q < HALF / 16; ++q) {
+    float x[16];
+#pragma unroll
+    for (int c = 0; c < 16; ++c) x[c] = __uint_as_float(s[q >> 1][16 * (q & 1) + c]);
+    const float a = max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), max3(x[6], x[7], x[8]));
+    const float b = max3(max3(x[9], x[10], x[11]), max3(x[12], x[13], x[14]), x[15]);
+    top = fmaxf(top, fmaf(fmaxf(a, b), factor(sl[q].k, fac), sl[q].lv));
+  }
+  return top;
+}
+// P = 2^(s - m) in f16 over the first half of the row's scores; returns l plus the row's share of the denominator.
+__device__ __forceinline__ float row_weights(uint32_t at_s, const uint32_t (&s)[2][32], const Slice* sl, float fac,
+                                             float m, float l) {
+#pragma unroll
+  for (int q = 0; q < HALF / 32; ++q) {
+    uint32_t pk[16];
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const Slice& k = sl[2 * q + hf];
+      const float f = factor(k.k, fac), d = k.lv - m;
+      const uint64_t f2 = pair2(f, f), d2 = pair2(d, d);
+      uint64_t sum = 0;
+#pragma unroll
+      for (int c = 0; c < 16; c += 2) {
+        float a, b;
+        unpair2(fma2(pair2(__uint_as_float(s[q][16 * hf + c]), __uint_as_float(s[q][16 * hf + c + 1])), f2, d2), a, b);
+        a = ex2(a);
+        b = ex2(b);
+        sum = add2(sum, pair2(a, b));
+        pk[8 * hf + c / 2] = pack2<__half>(a, b);
+      }
+      float a, b;
+      unpair2(sum, a, b);
+      l = fmaf(a + b, k.iv, l);
+    }
+    tmem_st16(at_s + 16 * q, pk);
+  }
+  return l;
+}
+// one lane of a converged warp; the compiler then keeps the products' operands in uniform registers
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(p));
+  return p != 0;
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const AttnParams p) {
@@ -125,7 +237,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
   __shared__ uint32_t s_tmem;
   __shared__ int s_pre[MAX_REQ + 1];
   __shared__ int s_wsum[PF_THREADS / 32];
-  const int t = threadIdx.x, lane = t & 31, w = t >> 5;
+  __shared__ Req s_req[KEPT_REQ];
+  const int t = threadIdx.x, lane = t & 31, w = __shfl_sync(0xffffffffu, t >> 5, 0);
   const uint32_t smem = (smem_u32(raw) + 1023) & ~1023u;
 
   // tiles before each request
@@ -134,7 +247,9 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
   for (int i = 0; i < per; ++i) {
     const int r = t * per + i;
     if (r >= p.n_req) break;
-    sum += (request(p, r, blockIdx.x == 0).q_len * p.g + ROWS - 1) / ROWS;
+    const Req x = request(p, r, blockIdx.x == 0);
+    if (p.n_req <= KEPT_REQ) s_req[r] = x;
+    sum += (x.q_len * p.g + ROWS - 1) / ROWS;
     s_pre[r + 1] = sum;
   }
   int inc = sum;
@@ -166,15 +281,15 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
     if (s_pre[mid] <= tile) r = mid;
     else b = mid;
   }
-  const Req x = request(p, r, false);
+  const Req x = p.n_req <= KEPT_REQ ? s_req[r] : request(p, r, false);
   const int row0 = (tile - s_pre[r]) * ROWS;
   const int n_here = min(ROWS, x.q_len * p.g - row0);
   const int behind = x.kv - x.q_len;
   const int lim_hi = behind + (row0 + n_here - 1) / p.g;         // last key that any row sees
-  const int n_tiles = lim_hi < 0 ? 0 : lim_hi / KT + 1;
+  const int n_tiles = lim_hi < 0 ? 0 : lim_hi / KT + 1, n_half = lim_hi < 0 ? 0 : lim_hi / HALF + 1;
   const bool two = n_here > GROUP_ROWS;
 
-  if (w == 12) {
+  if (w == MMA_WARP) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
                  "r"(512)
                  : "memory");
@@ -182,16 +297,19 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
   }
   if (t == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar.k_full[i], 4);
-      mbar_init(&bar.v_full[i], 4);
-      mbar_init(&bar.k_free[i], 1);
-      mbar_init(&bar.v_free[i], 1);
-      mbar_init(&bar.s_full[i], 1);
-      mbar_init(&bar.p_full[i], GROUP_ROWS);
+      mbar_init(&bar.k_full[i], CONVERTERS);
+      mbar_init(&bar.v_full[i], CONVERTERS);
+      mbar_init(&bar.k_free[i], two ? 2 : 1);           // both issuers
+      mbar_init(&bar.v_free[i], two ? 2 : 1);
+      mbar_init(&bar.drain[i], 1);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&bar.s_full[i][b], 1);
+        mbar_init(&bar.p_full[i][b], GROUP_ROWS);
+      }
+      mbar_init(&bar.o_done[i], 1);
       mbar_init(&bar.done[i], 1);
     }
     for (int i = 0; i < 4; ++i) mbar_init(&bar.meta[i], 1);
-    mbar_init(&bar.drain, 1);
     mbar_fence_init();
   }
 
@@ -200,65 +318,67 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
   int lim = -1;
   int64_t out_at = -1, lse_at = 0;
   if (w < 8) {
-    float v[8];
-    const bool live = t < n_here;
-    const T* q = static_cast<const T*>(p.q);
-    if (live) {
+    constexpr int LPR = D / 8, RPI = 32 / LPR;          // lanes of a row (16 bytes each), rows of an instruction
+    constexpr int N = 32 / RPI;
+    if (t < n_here) {
       const int tok = (row0 + t) / p.g, head = h * p.g + (row0 + t) % p.g;
       lim = behind + tok;
-      q += (int64_t)(x.q0 + tok) * p.q_row + head * p.q_head;
       out_at = (int64_t)(x.q0 + tok) * p.o_row + head * p.o_head;
       lse_at = (int64_t)(x.q0 + tok) * p.nq + head;
     }
-    const bool vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0;
-    auto load8 = [&](int e) {
-      if (!live) {
+    // the warp's 32 rows, RPI at a time, all loads in flight together
+    const int c = lane % LPR;
+    uint4 v[N];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = 0.0f;
-      } else if (vec) {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(q + e));
-        const uint32_t aw[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float2 f = unpack2<T>(aw[k]);
-          v[2 * k] = f.x;
-          v[2 * k + 1] = f.y;
+    for (int i = 0; i < N; ++i) {
+      const int n = 32 * w + RPI * i + lane / LPR;
+      v[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (n < n_here) {
+        const int tok = (row0 + n) / p.g, head = h * p.g + (row0 + n) % p.g;
+        const T* q = static_cast<const T*>(p.q) + (int64_t)(x.q0 + tok) * p.q_row + head * p.q_head + 8 * c;
+        if ((reinterpret_cast<uintptr_t>(q) & 15) == 0) {
+          v[i] = __ldg(reinterpret_cast<const uint4*>(q));
+        } else {
+          const unsigned short* e = reinterpret_cast<const unsigned short*>(q);
+          v[i] = make_uint4(__ldg(e) | ((uint32_t)__ldg(e + 1) << 16), __ldg(e + 2) | ((uint32_t)__ldg(e + 3) << 16),
+                            __ldg(e + 4) | ((uint32_t)__ldg(e + 5) << 16),
+                            __ldg(e + 6) | ((uint32_t)__ldg(e + 7) << 16));
         }
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = load_f<T>(q + e + k);
       }
-    };
+    }
     // the factor stays positive (a maximum is taken before it is applied); the sign goes to the query
-    float up = p.scale2 < 0.0f ? -1.0f : 1.0f;
+    const float sign = p.scale2 < 0.0f ? -1.0f : 1.0f;
     fac = fabsf(p.scale2);
-    if constexpr (!std::is_same<T, __half>::value) {
-      float top = 0.0f;
-      for (int e = 0; e < D; e += 8) {
-        load8(e);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(v[k]));
+    for (int i = 0; i < N; ++i) {
+      const uint32_t e[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+      float2 f[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) f[k] = unpack2<T>(e[k]);
+      float up = sign;
+      if constexpr (!std::is_same<T, __half>::value) {  // bf16: a power of two per row brings it into f16's range
+        float top = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top = max3(top, fabsf(f[k].x), fabsf(f[k].y));
+#pragma unroll
+        for (int o = 1; o < LPR; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const int k = min(126, 135 - (int)(__float_as_uint(top) >> 23));     // top * 2^k in [2^8, 2^9)
+        up *= __uint_as_float((uint32_t)(k + 127) << 23);
+        // to the thread that has the row
+        const int mine = __shfl_sync(0xffffffffu, k, (lane % RPI) * LPR);
+        if (lane / RPI == i) fac *= __uint_as_float((uint32_t)(127 - mine) << 23);
       }
-      const int k = min(126, 135 - (int)(__float_as_uint(top) >> 23));     // top * 2^k in [2^8, 2^9)
-      up *= __uint_as_float((uint32_t)(k + 127) << 23);
-      fac *= __uint_as_float((uint32_t)(127 - k) << 23);
+      const int row = 32 * (w & 3) + RPI * i + lane / LPR;
+      sts16(smem + L::Q + (w >> 2) * L::TILE + row * 128 + (c / 8) * L::BLOCK + (((c % 8) ^ (row & 7)) << 4),
+            pack2<__half>(f[0].x * up, f[0].y * up), pack2<__half>(f[1].x * up, f[1].y * up),
+            pack2<__half>(f[2].x * up, f[2].y * up), pack2<__half>(f[3].x * up, f[3].y * up));
     }
-    const int row = t & (GROUP_ROWS - 1);
-    const uint32_t dst = smem + L::Q + (t >> 7) * L::TILE + row * 128;
-#pragma unroll
-    for (int e = 0; e < D; e += 8) {
-      load8(e);
-      const int c = e / 8;
-      sts16(dst + (c / 8) * L::BLOCK + (((c % 8) ^ (row & 7)) << 4), pack2<__half>(v[0] * up, v[1] * up),
-            pack2<__half>(v[2] * up, v[3] * up), pack2<__half>(v[4] * up, v[5] * up),
-            pack2<__half>(v[6] * up, v[7] * up));
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    fence_proxy();
   }
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = s_tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
   bool ok = true;
 
   if (w < 8) {
@@ -268,139 +388,132 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
       const uint32_t at_s = tmem + ((uint32_t)(w & 3) << 21) + 128 * g2, at_o = at_s + 256;
       const int lim_first = behind + (row0 + GROUP_ROWS * g2) / p.g;
       float m = M_NONE, l = 0.0f;
-      uint32_t s[32];
-      for (int j = 0; j < n_tiles; ++j) {
-        ok = ok && mbar_wait(&bar.meta[j & 3], (j >> 2) & 1, PF_WAIT_NS);
-        ok = ok && mbar_wait(&bar.s_full[g2], j & 1, PF_WAIT_NS);
+      for (int i = 0; i < n_half; ++i) {
+        const int b = i & 1, j = i >> 1;
+        if (b == 0) ok = ok && wait_on(&bar.meta[j & 3], (j >> 2) & 1);
+        ok = ok && wait_on(&bar.s_full[g2][b], j & 1);
         if (!__all_sync(0xffffffffu, ok)) break;
         fence_after();
-        const Slice* sl = meta[j & 3];
-        const bool masked = j * KT + KT - 1 > lim_first;
-        const int last = lim - j * KT;                  // columns past it are not seen
-        float top = -INFINITY;
-#pragma unroll
-        for (int c0 = 0; c0 < KT; c0 += 32) {
-          tmem_ld32(at_s + c0, s);
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            float mx = -INFINITY;
-#pragma unroll
-            for (int c = 0; c < 16; ++c) {
-              float v = __uint_as_float(s[16 * hf + c]);
-              if (masked && c0 + 16 * hf + c > last) v = -INFINITY;
-              mx = fmaxf(mx, v);
-            }
-            const Slice& q = sl[c0 / 16 + hf];
-            top = fmaxf(top, fmaf(mx, q.k * fac, q.lv));
-          }
-        }
+        const Slice* sl = meta[j & 3] + (HALF / 16) * b;
+        const bool masked = i * HALF + HALF - 1 > lim_first;
+        const int last = lim - i * HALF;                // columns past it are not seen
+        const uint32_t at = at_s + HALF * b;
+        uint32_t s[2][32];
+        tmem_ld32(at, s[0]);
+        tmem_ld32(at + 32, s[1]);
+        tmem_wait_ld(s[0]);
+        tmem_wait_ld(s[1]);
+        if (masked) mask_row(s, last);
+        const float top = row_max(s, sl, fac);
         if (__any_sync(0xffffffffu, top > m + 8.0f)) {
           const float m1 = fmaxf(m, top), keep = ex2(m - m1);
           m = m1;
           l *= keep;
-          if (j > 0) {                                  // S of this tile is complete, so the products before it are
+          if (i > 0) {
+            ok = wait_on(&bar.o_done[g2], (i - 1) & 1);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            fence_after();
 #pragma unroll 1
-            for (int c0 = 0; c0 < D; c0 += 32) {
-              tmem_ld32(at_o + c0, s);
+            for (int c0 = 0; c0 < D; c0 += 16) {
+              uint32_t o[16];
+              tmem_ld16(at_o + c0, o);
 #pragma unroll
-              for (int c = 0; c < 32; ++c) s[c] = __float_as_uint(__uint_as_float(s[c]) * keep);
-              tmem_st32(at_o + c0, s);
+              for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * keep);
+              tmem_st16(at_o + c0, o);
             }
           }
         }
-#pragma unroll
-        for (int c0 = 0; c0 < KT; c0 += 32) {
-          tmem_ld32(at_s + c0, s);
-          uint32_t pk[16];
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            const Slice& q = sl[c0 / 16 + hf];
-            const float f = q.k * fac, d = q.lv - m;
-            float part = 0.0f;
-#pragma unroll
-            for (int c = 0; c < 16; c += 2) {
-              float a = ex2(fmaf(__uint_as_float(s[16 * hf + c]), f, d));
-              float b = ex2(fmaf(__uint_as_float(s[16 * hf + c + 1]), f, d));
-              if (masked) {
-                if (c0 + 16 * hf + c > last) a = 0.0f;
-                if (c0 + 16 * hf + c + 1 > last) b = 0.0f;
-              }
-              part += a + b;
-              pk[8 * hf + c / 2] = pack2<__half>(a, b);
-            }
-            l = fmaf(part, q.iv, l);
-          }
-          tmem_st16(at_s + c0 / 2, pk);
-        }
+        l = row_weights(at, s, sl, fac, m, l);
         tmem_wait_st();
         fence_before();
-        mbar_arrive(&bar.p_full[g2]);
+        mbar_arrive(&bar.p_full[g2][b]);
       }
+      uint32_t s[32];
       if (n_tiles > 0) {
-        ok = ok && mbar_wait(&bar.done[g2], 0, PF_WAIT_NS);
+        ok = ok && wait_on(&bar.done[g2], 0);
         ok = __all_sync(0xffffffffu, ok);
         fence_after();
       }
-      T* out = static_cast<T*>(p.out) + out_at;
-      const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+      // The warp's 32 rows go through its part of the query tile (no product reads it any more), so that a
+      // store instruction writes whole rows.
       const float inv = l > 0.0f ? __frcp_rn(l) : l;    // no key: 0, and NaN stays NaN
+      const int row = t & (GROUP_ROWS - 1);
+      const uint32_t stage = smem + L::Q + g2 * L::TILE;
 #pragma unroll 1
       for (int c0 = 0; c0 < D; c0 += 32) {
         if (n_tiles > 0 && ok) {
           tmem_ld32(at_o + c0, s);
+          tmem_wait_ld(s);
         } else {
 #pragma unroll
           for (int c = 0; c < 32; ++c) s[c] = 0u;
         }
-        if (out_at >= 0) {
 #pragma unroll
-          for (int c = 0; c < 32; c += 8) {
-            uint32_t o[4];
+        for (int c = 0; c < 32; c += 8) {
+          uint32_t o[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              o[k] = l == 0.0f ? 0u
-                               : pack2<T>(__uint_as_float(s[c + 2 * k]) * inv, __uint_as_float(s[c + 2 * k + 1]) * inv);
-            if (vec) {
-              *reinterpret_cast<uint4*>(out + c0 + c) = make_uint4(o[0], o[1], o[2], o[3]);
-            } else {
-              const T* e = reinterpret_cast<const T*>(o);
+          for (int k = 0; k < 4; ++k)
+            o[k] = l == 0.0f ? 0u
+                             : pack2<T>(__uint_as_float(s[c + 2 * k]) * inv, __uint_as_float(s[c + 2 * k + 1]) * inv);
+          const int x = (c0 + c) / 8;
+          sts16(stage + row * 128 + (x / 8) * L::BLOCK + (((x % 8) ^ (row & 7)) << 4), o[0], o[1], o[2], o[3]);
+        }
+      }
+      __syncwarp();
+      constexpr int LPR = D / 8, RPI = 32 / LPR;
+#pragma unroll 4
+      for (int i = 0; i < 32 / RPI; ++i) {
+        const int src = RPI * i + lane / LPR, c = lane % LPR, n = 32 * (w & 3) + src;
+        const int64_t at = __shfl_sync(0xffffffffu, out_at, src);
+        uint4 v;
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                     : "r"(stage + n * 128 + (c / 8) * L::BLOCK + (((c % 8) ^ (n & 7)) << 4))
+                     : "memory");
+        if (at < 0) continue;
+        T* out = static_cast<T*>(p.out) + at + 8 * c;
+        if ((reinterpret_cast<uintptr_t>(out) & 15) == 0) {
+          *reinterpret_cast<uint4*>(out) = v;
+        } else {
+          const uint32_t e[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-              for (int k = 0; k < 8; ++k) out[c0 + c + k] = e[k];
-            }
+          for (int k = 0; k < 4; ++k) {
+            const T* pair = reinterpret_cast<const T*>(&e[k]);
+            out[2 * k] = pair[0];
+            out[2 * k + 1] = pair[1];
           }
         }
       }
       if (out_at >= 0 && p.lse) p.lse[lse_at] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * LN2;
     }
-  } else if (w < 12) {
+  } else if (w < MMA_WARP) {
     // ---- converters: e4m3 pages -> f16 operand tiles -------------------------
     constexpr int PIECES = D / 16;                      // 16-byte pieces of a key row
-    constexpr int KEYS = 128 / PIECES;                  // keys that the 128 threads cover at once
+    constexpr int KEYS = 32 * CONVERTERS / PIECES;      // keys that the threads cover at once
     constexpr int N = KT / KEYS;                        // pieces per thread
     const int ct = t - 256, piece = ct % PIECES, key0 = ct / PIECES;
     uint4 kr[N], vr[N];
-    // a lane's page and scales of slice `lane` of a tile
-    auto page_of = [&](int j) {
-      int page = -1;
-      const int key = j * KT + (lane & (SLICES - 1)) * 16;
-      if (key <= lim_hi) {
-        page = __ldg(p.tables + (int64_t)r * p.t_stride + (key >> p.page_log2));
-        if (page < 0 || page >= p.n_pages) {
-          if (p.status) atomicOr(p.status, HC_ERR_RANGE);
-          page = -1;
-        }
-      }
-      return page;
+    // page of a 16-key slice of a tile, -1 where there is none
+    auto page_of = [&](int j, int slice) {
+      const int key = j * KT + slice * 16;
+      return key <= lim_hi ? __ldg(p.tables + (int64_t)r * p.t_stride + (key >> p.page_log2)) : -1;
     };
-    auto load = [&](const uint8_t* pool, int j, int page, uint4 (&v)[N]) {
+    // A thread's pieces lie in N slices; it reads their pages itself, a tile
+    // ahead: shuffles between the loads made each wait for the one before.
+    int pg[N];
+    auto pages = [&](int j) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) pg[i] = page_of(j, (key0 + KEYS * i) / 16);
+    };
+    auto load = [&](const uint8_t* pool, int j, uint4 (&v)[N]) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int kk = key0 + KEYS * i, key = j * KT + kk;
-        const int pg = __shfl_sync(0xffffffffu, page, kk / 16);
+        const int key = j * KT + key0 + KEYS * i;
         v[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (pg >= 0 && key <= lim_hi)
+        if (pg[i] >= 0 && pg[i] < p.n_pages && key <= lim_hi)
           v[i] = __ldg(reinterpret_cast<const uint4*>(
-              pool + ((((int64_t)pg * p.nkv + h) << p.page_log2) + (key & ((1 << p.page_log2) - 1))) * D + 16 * piece));
+              pool + ((((int64_t)pg[i] * p.nkv + h) << p.page_log2) + (key & ((1 << p.page_log2) - 1))) * D +
+              16 * piece));
       }
     };
     auto store = [&](uint32_t dst, const uint4 (&v)[N]) {
@@ -424,104 +537,140 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
           else sts16(at, f[0], f[1], f[2], f[3]);
         }
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
     };
-    int page = -1;
+    // The next tile's bytes are loaded while this one's are converted.  The
+    // issuers order these stores before their products: a proxy fence here
+    // would wait for the loads in flight.  Lane l of the first warp has slice
+    // l's scales.
+    int at = -1, next = -1;
+    float ks = 0.0f, vs = 1.0f;
+    auto load_scales = [&]() {
+      ks = 0.0f;
+      vs = 1.0f;
+      if (at >= p.n_pages) at = -1;
+      if (at >= 0) {
+        ks = __ldg(p.ks + (int64_t)at * p.nkv + h);
+        vs = __ldg(p.vs + (int64_t)at * p.nkv + h);
+      }
+    };
+    const bool scales = w == 8 && lane < SLICES;
     if (n_tiles > 0) {
-      page = page_of(0);
-      load(p.kp, 0, page, kr);
-      load(p.vp, 0, page, vr);
+      pages(0);
+      load(p.kp, 0, kr);
+      load(p.vp, 0, vr);
+      if (scales) {
+        at = page_of(0, lane);
+        if (n_tiles > 1) next = page_of(1, lane);
+        load_scales();
+      }
+      if (n_tiles > 1) pages(1);
     }
     for (int j = 0; j < n_tiles; ++j) {
       const int st = j & 1;
-      Slice mine = {0.0f, 0.0f, 0.0f};
-      if (w == 8 && lane < SLICES && page >= 0) {
-        const float a = __ldg(p.ks + (int64_t)page * p.nkv + h);
-        const float b = fmaxf(__ldg(p.vs + (int64_t)page * p.nkv + h), 1e-30f);
-        mine.k = a;
-        mine.lv = __log2f(b);
-        mine.iv = __frcp_rn(b);
-      } else if (page < 0) {
-        mine.lv = -INFINITY;                            // no page: no weight
-      }
-      const int next = j + 1 < n_tiles ? page_of(j + 1) : -1;
-      if (j >= 2) ok = ok && mbar_wait(&bar.k_free[st], ((j >> 1) - 1) & 1, PF_WAIT_NS);
+      if (j >= 2) ok = ok && wait_on(&bar.k_free[st], ((j >> 1) - 1) & 1);
       if (!__all_sync(0xffffffffu, ok)) break;
-      if (w == 8 && lane < SLICES) meta[j & 3][lane] = mine;
+      if (scales) {
+        Slice mine = {ks, -INFINITY, 0.0f};             // no page: no weight
+        if (at >= 0) {
+          const float b = fmaxf(vs, 1e-30f);
+          mine.lv = __log2f(b);
+          mine.iv = __frcp_rn(b);
+        } else if (j * KT + lane * 16 <= lim_hi && p.status) {
+          atomicOr(p.status, HC_ERR_RANGE);
+        }
+        meta[j & 3][lane] = mine;
+      }
       store(smem + L::K + st * L::TILE, kr);
       if (lane == 0) {                                  // after store()'s __syncwarp
         if (w == 8) mbar_arrive(&bar.meta[j & 3]);
         mbar_arrive(&bar.k_full[st]);
       }
-      if (j + 1 < n_tiles) load(p.kp, j + 1, next, kr);
-      if (j >= 2) ok = ok && mbar_wait(&bar.v_free[st], ((j >> 1) - 1) & 1, PF_WAIT_NS);
+      if (j + 1 < n_tiles) load(p.kp, j + 1, kr);
+      if (j >= 2) ok = ok && wait_on(&bar.v_free[st], ((j >> 1) - 1) & 1);
       if (!__all_sync(0xffffffffu, ok)) break;
       store(smem + L::V + st * L::TILE, vr);
       if (lane == 0) mbar_arrive(&bar.v_full[st]);
-      if (j + 1 < n_tiles) load(p.vp, j + 1, next, vr);
-      page = next;
-    }
-  } else if (n_tiles > 0) {
-    // ---- MMA: one thread issues -----------------------------------------------
-    if (lane == 0) {
-      constexpr uint32_t id_s = pf_idesc(KT, 0), id_o = pf_idesc(D, 1);
-      auto scores = [&](int g2, int j) {
-        const uint32_t q = smem + L::Q + g2 * L::TILE, k = smem + L::K + (j & 1) * L::TILE;
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          const uint32_t at = (i / 4) * L::BLOCK + (i % 4) * 32;
-          mma_ss(tmem + 128 * g2, sw128_desc(q + at, 16, 1024), sw128_desc(k + at, 16, 1024), id_s, i > 0);
+      if (j + 1 < n_tiles) {
+        load(p.vp, j + 1, vr);
+        if (scales) {
+          at = next;
+          load_scales();
         }
-      };
-      auto values = [&](int g2, int j) {
-        const uint32_t v = smem + L::V + (j & 1) * L::TILE;
-#pragma unroll
-        for (int i = 0; i < KT / 16; ++i)
-          mma_ts(tmem + 256 + 128 * g2, tmem + 128 * g2 + 8 * i, sw128_desc(v + 2048 * i, L::BLOCK, 1024), id_o,
-                 j > 0 || i > 0);
-      };
-      ok = mbar_wait(&bar.k_full[0], 0, PF_WAIT_NS);
-      if (ok) {
-        fence_after();
-        scores(0, 0);
-        mma_commit(&bar.s_full[0]);
-        if (two) {
-          scores(1, 0);
-          mma_commit(&bar.s_full[1]);
-        }
-        mma_commit(&bar.k_free[0]);
-        for (int j = 0; j < n_tiles && ok; ++j) {
-          const bool more = j + 1 < n_tiles;
-          ok = mbar_wait(&bar.v_full[j & 1], (j >> 1) & 1, PF_WAIT_NS);
-          if (more) ok = ok && mbar_wait(&bar.k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, PF_WAIT_NS);
-          for (int g2 = 0; g2 < (two ? 2 : 1) && ok; ++g2) {
-            ok = mbar_wait(&bar.p_full[g2], j & 1, PF_WAIT_NS);
-            if (!ok) break;
-            fence_after();
-            values(g2, j);
-            if (more) {
-              scores(g2, j + 1);
-              mma_commit(&bar.s_full[g2]);
-            } else {
-              mma_commit(&bar.done[g2]);
-            }
-          }
-          if (!ok) break;
-          mma_commit(&bar.v_free[j & 1]);
-          if (more) mma_commit(&bar.k_free[(j + 1) & 1]);
+        if (j + 2 < n_tiles) {
+          pages(j + 2);
+          if (scales) next = page_of(j + 2, lane);
         }
       }
+    }
+  } else if (n_tiles > 0) {
+    // ---- MMA: one thread a group ----------------------------------------------
+    // Half i uses buffer i % 2 and stage (i / 2) % 2.  The loops stay rolled:
+    // unrolled over the stages, the issuers' code pushed the other roles' out of
+    // the instruction caches.
+    if (elect_one() && (w == MMA_WARP || two)) {
+      constexpr uint32_t id_s = pf_idesc(HALF, 0), id_o = pf_idesc(D, 1);
+      const int g2 = w - MMA_WARP;
+      const uint32_t t_s = tmem + 128 * g2, t_o = t_s + 256;
+      const uint64_t d_q = sw128_desc(smem + L::Q + g2 * L::TILE, 16, 1024);
+      const uint64_t d_k = sw128_desc(smem + L::K, 16, 1024), d_v = sw128_desc(smem + L::V, L::BLOCK, 1024);
+      auto place = [](int i) {                          // of half i among the two stages, in descriptor units
+        return (uint64_t)((((i >> 1) & 1) * L::TILE + (i & 1) * (HALF * 128)) >> 4);
+      };
+      auto scores = [&](int i) {
+        uint64_t a = d_q, b = d_k + place(i);
+        const uint32_t d = t_s + HALF * (i & 1);
+#pragma unroll 1
+        for (int e = 0; e < D / 64; ++e) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mma_ss(d, a + 2 * k, b + 2 * k, id_s, e + k);
+          a += L::BLOCK >> 4;
+          b += L::BLOCK >> 4;
+        }
+        mma_commit(&bar.s_full[g2][i & 1]);
+      };
+      ok = wait_on(&bar.k_full[0], 0);
+      if (ok) {
+        fence_proxy();
+        fence_after();
+        scores(0);
+        if (n_half > 1) scores(1);
+        mma_commit(&bar.k_free[0]);
+#pragma unroll 1
+        for (int i = 0; i < n_half; ++i) {
+          const int st = (i >> 1) & 1;
+          const bool more = i + 2 < n_half;
+          if ((i & 1) == 0) {
+            ok = wait_on(&bar.v_full[st], (i >> 2) & 1);
+            if (more) ok = ok && wait_on(&bar.k_full[st ^ 1], ((i + 2) >> 2) & 1);
+            fence_proxy();
+          }
+          ok = ok && wait_on(&bar.p_full[g2][i & 1], st);
+          if (!ok) break;
+          fence_after();
+          const uint64_t b = d_v + place(i);
+#pragma unroll
+          for (int e = 0; e < HALF / 16; ++e)
+            mma_ts(t_o, t_s + HALF * (i & 1) + 8 * e, b + 128 * e, id_o, i + e);
+          mma_commit(&bar.o_done[g2]);
+          if (i & 1) mma_commit(&bar.v_free[st]);
+          if (more) {
+            scores(i + 2);
+            if (i & 1) mma_commit(&bar.k_free[st ^ 1]);
+          }
+        }
+        if (ok) mma_commit(&bar.done[g2]);
+      }
       // every product that was issued has completed before the CTA gives up its memory
-      mma_commit(&bar.drain);
-      mbar_wait(&bar.drain, 0, PF_WAIT_NS);
+      mma_commit(&bar.drain[g2]);
+      wait_on(&bar.drain[g2], 0);
     }
   }
   if (!ok && p.status) atomicOr(p.status, HC_ERR_TIMEOUT);
   fence_before();
   __syncthreads();
   fence_after();
-  if (w == 12)
+  if (w == MMA_WARP)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
