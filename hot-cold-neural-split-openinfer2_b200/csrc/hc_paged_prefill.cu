@@ -27,8 +27,9 @@
 namespace hca8 {
 
 constexpr int CONVERTERS = 4;          // warps
-constexpr int PF_THREADS = 256 + 32 * CONVERTERS + 64;      // 8 softmax warps, the converters, an MMA warp per group
-constexpr int MMA_WARP = 8 + CONVERTERS;
+constexpr int MMA_WARP = 8 + CONVERTERS;                // two, one for each group
+constexpr int SCALE_WARP = MMA_WARP + 2;
+constexpr int PF_THREADS = 32 * (SCALE_WARP + 1);       // and 8 softmax warps
 constexpr int GROUP_ROWS = 128;
 constexpr int ROWS = 2 * GROUP_ROWS;
 constexpr int KT = 128;                // keys per converted tile
@@ -161,8 +162,9 @@ struct Bars {
   uint64_t p_full[2][2];               // group -> MMA: the buffer's weights are written
   uint64_t o_done[2];                  // MMA -> group: a half's product is in O
   uint64_t done[2];                    // MMA -> group: all products are
-  uint64_t meta[4];                    // converters -> groups: a tile's scales
+  uint64_t meta[4];                    // scale warp -> groups: a tile's scales
   uint64_t drain[2];
+  uint64_t q_full[2];                  // group -> MMA: its queries are in place
 };
 
 // Shared by the roles of one CTA.
@@ -302,6 +304,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
       mbar_init(&bar.k_free[i], two ? 2 : 1);           // both issuers
       mbar_init(&bar.v_free[i], two ? 2 : 1);
       mbar_init(&bar.drain[i], 1);
+      mbar_init(&bar.q_full[i], GROUP_ROWS);
       for (int b = 0; b < 2; ++b) {
         mbar_init(&bar.s_full[i][b], 1);
         mbar_init(&bar.p_full[i][b], GROUP_ROWS);
@@ -313,68 +316,6 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
     mbar_fence_init();
   }
 
-  // queries: a thread has a row
-  float fac = 0.0f;
-  int lim = -1;
-  int64_t out_at = -1, lse_at = 0;
-  if (w < 8) {
-    constexpr int LPR = D / 8, RPI = 32 / LPR;          // lanes of a row (16 bytes each), rows of an instruction
-    constexpr int N = 32 / RPI;
-    if (t < n_here) {
-      const int tok = (row0 + t) / p.g, head = h * p.g + (row0 + t) % p.g;
-      lim = behind + tok;
-      out_at = (int64_t)(x.q0 + tok) * p.o_row + head * p.o_head;
-      lse_at = (int64_t)(x.q0 + tok) * p.nq + head;
-    }
-    // the warp's 32 rows, RPI at a time, all loads in flight together
-    const int c = lane % LPR;
-    uint4 v[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int n = 32 * w + RPI * i + lane / LPR;
-      v[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (n < n_here) {
-        const int tok = (row0 + n) / p.g, head = h * p.g + (row0 + n) % p.g;
-        const T* q = static_cast<const T*>(p.q) + (int64_t)(x.q0 + tok) * p.q_row + head * p.q_head + 8 * c;
-        if ((reinterpret_cast<uintptr_t>(q) & 15) == 0) {
-          v[i] = __ldg(reinterpret_cast<const uint4*>(q));
-        } else {
-          const unsigned short* e = reinterpret_cast<const unsigned short*>(q);
-          v[i] = make_uint4(__ldg(e) | ((uint32_t)__ldg(e + 1) << 16), __ldg(e + 2) | ((uint32_t)__ldg(e + 3) << 16),
-                            __ldg(e + 4) | ((uint32_t)__ldg(e + 5) << 16),
-                            __ldg(e + 6) | ((uint32_t)__ldg(e + 7) << 16));
-        }
-      }
-    }
-    // the factor stays positive (a maximum is taken before it is applied); the sign goes to the query
-    const float sign = p.scale2 < 0.0f ? -1.0f : 1.0f;
-    fac = fabsf(p.scale2);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const uint32_t e[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-      float2 f[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) f[k] = unpack2<T>(e[k]);
-      float up = sign;
-      if constexpr (!std::is_same<T, __half>::value) {  // bf16: a power of two per row brings it into f16's range
-        float top = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) top = max3(top, fabsf(f[k].x), fabsf(f[k].y));
-#pragma unroll
-        for (int o = 1; o < LPR; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const int k = min(126, 135 - (int)(__float_as_uint(top) >> 23));     // top * 2^k in [2^8, 2^9)
-        up *= __uint_as_float((uint32_t)(k + 127) << 23);
-        // to the thread that has the row
-        const int mine = __shfl_sync(0xffffffffu, k, (lane % RPI) * LPR);
-        if (lane / RPI == i) fac *= __uint_as_float((uint32_t)(127 - mine) << 23);
-      }
-      const int row = 32 * (w & 3) + RPI * i + lane / LPR;
-      sts16(smem + L::Q + (w >> 2) * L::TILE + row * 128 + (c / 8) * L::BLOCK + (((c % 8) ^ (row & 7)) << 4),
-            pack2<__half>(f[0].x * up, f[0].y * up), pack2<__half>(f[1].x * up, f[1].y * up),
-            pack2<__half>(f[2].x * up, f[2].y * up), pack2<__half>(f[3].x * up, f[3].y * up));
-    }
-    fence_proxy();
-  }
   fence_before();
   __syncthreads();
   fence_after();
@@ -385,6 +326,88 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
     // ---- softmax: group g2, one row a thread --------------------------------
     const int g2 = w >> 2;
     if (g2 == 0 || two) {
+      // this thread's row; queries and outputs move LPR lanes to a row, RPI rows an instruction
+      constexpr int LPR = D / 8, RPI = 32 / LPR;
+      const int c = lane % LPR, row = t & (GROUP_ROWS - 1);
+      const uint32_t q_tile = smem + L::Q + g2 * L::TILE;
+      int lim = -1;
+      int64_t q_at = -1, out_at = -1, lse_at = 0;
+      if (t < n_here) {
+        const int tok = (row0 + t) / p.g, head = h * p.g + (row0 + t) - tok * p.g;
+        lim = behind + tok;
+        q_at = (int64_t)(x.q0 + tok) * p.q_row + head * p.q_head;
+        out_at = (int64_t)(x.q0 + tok) * p.o_row + head * p.o_head;
+        lse_at = (int64_t)(x.q0 + tok) * p.nq + head;
+      }
+      // the factor stays positive (a maximum is taken before it is applied); the sign goes to the query
+      const float sign = p.scale2 < 0.0f ? -1.0f : 1.0f;
+      float fac = fabsf(p.scale2);
+      const bool q_vec = (reinterpret_cast<uintptr_t>(p.q) & 15) == 0 && p.q_row % 8 == 0 && p.q_head % 8 == 0;
+      auto spot = [&](int to) {                         // of piece c of row `to` in the operand tile
+        return q_tile + to * 128 + (c / 8) * L::BLOCK + (((c % 8) ^ (to & 7)) << 4);
+      };
+      auto place_query = [&](int i, uint4 v) {          // converts and stores pieces of rows RPI i ..
+        const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+        uint32_t f[4];
+        float up = sign;
+        if constexpr (!std::is_same<T, __half>::value) {         // bf16: a power of two brings a row into f16's range
+          float top = 0.0f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 a = unpack2<T>(e[k]);
+            top = max3(top, fabsf(a.x), fabsf(a.y));
+          }
+#pragma unroll
+          for (int o = 1; o < LPR; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const int k = min(126, 135 - (int)(__float_as_uint(top) >> 23));       // top * 2^k in [2^8, 2^9)
+          up *= __uint_as_float((uint32_t)(k + 127) << 23);
+          const int mine = __shfl_sync(0xffffffffu, k, (lane % RPI) * LPR);      // to the thread that has the row
+          if (lane / RPI == i) fac *= __uint_as_float((uint32_t)(127 - mine) << 23);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 a = unpack2<T>(e[k]);
+          f[k] = pack2<__half>(a.x * up, a.y * up);
+        }
+        sts16(spot(32 * (w & 3) + RPI * i + lane / LPR), f[0], f[1], f[2], f[3]);
+      };
+      if (q_vec && std::is_same<T, __half>::value && sign > 0.0f) {              // f16 as it is: straight into the tile
+#pragma unroll 4
+        for (int i = 0; i < 32 / RPI; ++i) {
+          const int src = RPI * i + lane / LPR;
+          const int64_t at = __shfl_sync(0xffffffffu, q_at, src);
+          const T* q = static_cast<const T*>(p.q) + (at >= 0 ? at : 0) + 8 * c;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(spot(32 * (w & 3) + src)), "l"(q),
+                       "r"(at >= 0 ? 16 : 0)
+                       : "memory");
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+      } else if (q_vec) {
+        uint4 v[32 / RPI];
+#pragma unroll
+        for (int i = 0; i < 32 / RPI; ++i) {
+          const int64_t at = __shfl_sync(0xffffffffu, q_at, RPI * i + lane / LPR);
+          v[i] = make_uint4(0u, 0u, 0u, 0u);
+          if (at >= 0) v[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + at + 8 * c));
+        }
+#pragma unroll
+        for (int i = 0; i < 32 / RPI; ++i) place_query(i, v[i]);
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < 32 / RPI; ++i) {
+          const int64_t at = __shfl_sync(0xffffffffu, q_at, RPI * i + lane / LPR);
+          uint32_t e[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+          if (at >= 0) {
+            const unsigned short* q = reinterpret_cast<const unsigned short*>(static_cast<const T*>(p.q) + at + 8 * c);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) e[k] = __ldg(q + k);
+          }
+          place_query(i, make_uint4(e[0] | (e[1] << 16), e[2] | (e[3] << 16), e[4] | (e[5] << 16), e[6] | (e[7] << 16)));
+        }
+      }
+      fence_proxy();
+      mbar_arrive(&bar.q_full[g2]);
+
       const uint32_t at_s = tmem + ((uint32_t)(w & 3) << 21) + 128 * g2, at_o = at_s + 256;
       const int lim_first = behind + (row0 + GROUP_ROWS * g2) / p.g;
       float m = M_NONE, l = 0.0f;
@@ -437,8 +460,6 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
       // The warp's 32 rows go through its part of the query tile (no product reads it any more), so that a
       // store instruction writes whole rows.
       const float inv = l > 0.0f ? __frcp_rn(l) : l;    // no key: 0, and NaN stays NaN
-      const int row = t & (GROUP_ROWS - 1);
-      const uint32_t stage = smem + L::Q + g2 * L::TILE;
 #pragma unroll 1
       for (int c0 = 0; c0 < D; c0 += 32) {
         if (n_tiles > 0 && ok) {
@@ -456,19 +477,18 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
             o[k] = l == 0.0f ? 0u
                              : pack2<T>(__uint_as_float(s[c + 2 * k]) * inv, __uint_as_float(s[c + 2 * k + 1]) * inv);
           const int x = (c0 + c) / 8;
-          sts16(stage + row * 128 + (x / 8) * L::BLOCK + (((x % 8) ^ (row & 7)) << 4), o[0], o[1], o[2], o[3]);
+          sts16(q_tile + row * 128 + (x / 8) * L::BLOCK + (((x % 8) ^ (row & 7)) << 4), o[0], o[1], o[2], o[3]);
         }
       }
       __syncwarp();
-      constexpr int LPR = D / 8, RPI = 32 / LPR;
 #pragma unroll 4
       for (int i = 0; i < 32 / RPI; ++i) {
-        const int src = RPI * i + lane / LPR, c = lane % LPR, n = 32 * (w & 3) + src;
+        const int src = RPI * i + lane / LPR, n = 32 * (w & 3) + src;
         const int64_t at = __shfl_sync(0xffffffffu, out_at, src);
         uint4 v;
         asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                      : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                     : "r"(stage + n * 128 + (c / 8) * L::BLOCK + (((c % 8) ^ (n & 7)) << 4))
+                     : "r"(q_tile + n * 128 + (c / 8) * L::BLOCK + (((c % 8) ^ (n & 7)) << 4))
                      : "memory");
         if (at < 0) continue;
         T* out = static_cast<T*>(p.out) + at + 8 * c;
@@ -476,9 +496,10 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
           *reinterpret_cast<uint4*>(out) = v;
         } else {
           const uint32_t e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
+#pragma unroll 1
           for (int k = 0; k < 4; ++k) {
-            const T* pair = reinterpret_cast<const T*>(&e[k]);
+            const uint32_t u = k == 0 ? e[0] : k == 1 ? e[1] : k == 2 ? e[2] : e[3];
+            const T* pair = reinterpret_cast<const T*>(&u);
             out[2 * k] = pair[0];
             out[2 * k + 1] = pair[1];
           }
@@ -493,28 +514,40 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
     constexpr int N = KT / KEYS;                        // pieces per thread
     const int ct = t - 256, piece = ct % PIECES, key0 = ct / PIECES;
     uint4 kr[N], vr[N];
-    // page of a 16-key slice of a tile, -1 where there is none
-    auto page_of = [&](int j, int slice) {
-      const int key = j * KT + slice * 16;
-      return key <= lim_hi ? __ldg(p.tables + (int64_t)r * p.t_stride + (key >> p.page_log2)) : -1;
-    };
+    // Page of the slice that holds a key.  Keys behind lim_hi read the page of
+    // lim_hi: their bytes are replaced before they are converted.
+    const int32_t* table = p.tables + (int64_t)r * p.t_stride;
+    auto page_of = [&](int key) { return __ldg(table + (min(key, lim_hi) >> p.page_log2)); };
     // A thread's pieces lie in N slices; it reads their pages itself, a tile
     // ahead: shuffles between the loads made each wait for the one before.
+    // Every load is unconditional, from an address inside the pool.
+    const uint32_t page_bytes = (uint32_t)D << p.page_log2, in_page = ((uint32_t)1 << p.page_log2) - 1;
     int pg[N];
     auto pages = [&](int j) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) pg[i] = page_of(j, (key0 + KEYS * i) / 16);
+      for (int i = 0; i < N; ++i) pg[i] = page_of(j * KT + key0 + KEYS * i);
     };
     auto load = [&](const uint8_t* pool, int j, uint4 (&v)[N]) {
+      const uint8_t* base = pool + 16 * piece;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int key = j * KT + key0 + KEYS * i;
-        v[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (pg[i] >= 0 && pg[i] < p.n_pages && key <= lim_hi)
-          v[i] = __ldg(reinterpret_cast<const uint4*>(
-              pool + ((((int64_t)pg[i] * p.nkv + h) << p.page_log2) + (key & ((1 << p.page_log2) - 1))) * D +
-              16 * piece));
+        const uint32_t head = (uint32_t)((unsigned)pg[i] < (unsigned)p.n_pages ? pg[i] : 0) * p.nkv + h;
+        const uint32_t key = (uint32_t)(j * KT + key0 + KEYS * i) & in_page;
+        v[i] = __ldg(reinterpret_cast<const uint4*>(base + (uint64_t)head * page_bytes + key * D));
       }
+    };
+    // pieces of tile j without a page or behind lim_hi become zeros
+    uint32_t lost = 0, lost_next = 0;                   // pieces whose page is not in the pool
+    auto lose = [&]() {
+      lost_next = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) lost_next |= (unsigned)pg[i] < (unsigned)p.n_pages ? 0u : 1u << i;
+    };
+    auto blank = [&](int j, uint4 (&v)[N]) {
+      if (j + 1 < n_tiles && !__any_sync(0xffffffffu, lost != 0)) return;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (((lost >> i) & 1) || j * KT + key0 + KEYS * i > lim_hi) v[i] = make_uint4(0u, 0u, 0u, 0u);
     };
     auto store = [&](uint32_t dst, const uint4 (&v)[N]) {
       // a lane's two 16-byte halves in an order that spreads eight lanes over all banks
@@ -541,67 +574,73 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
     };
     // The next tile's bytes are loaded while this one's are converted.  The
     // issuers order these stores before their products: a proxy fence here
-    // would wait for the loads in flight.  Lane l of the first warp has slice
-    // l's scales.
-    int at = -1, next = -1;
-    float ks = 0.0f, vs = 1.0f;
-    auto load_scales = [&]() {
-      ks = 0.0f;
-      vs = 1.0f;
-      if (at >= p.n_pages) at = -1;
-      if (at >= 0) {
-        ks = __ldg(p.ks + (int64_t)at * p.nkv + h);
-        vs = __ldg(p.vs + (int64_t)at * p.nkv + h);
-      }
-    };
-    const bool scales = w == 8 && lane < SLICES;
+    // would wait for the loads in flight.
     if (n_tiles > 0) {
       pages(0);
       load(p.kp, 0, kr);
       load(p.vp, 0, vr);
-      if (scales) {
-        at = page_of(0, lane);
-        if (n_tiles > 1) next = page_of(1, lane);
-        load_scales();
-      }
-      if (n_tiles > 1) pages(1);
+      lose();
+      lost = lost_next;
+      pages(1);
     }
     for (int j = 0; j < n_tiles; ++j) {
       const int st = j & 1;
       if (j >= 2) ok = ok && wait_on(&bar.k_free[st], ((j >> 1) - 1) & 1);
       if (!__all_sync(0xffffffffu, ok)) break;
-      if (scales) {
-        Slice mine = {ks, -INFINITY, 0.0f};             // no page: no weight
-        if (at >= 0) {
-          const float b = fmaxf(vs, 1e-30f);
-          mine.lv = __log2f(b);
-          mine.iv = __frcp_rn(b);
-        } else if (j * KT + lane * 16 <= lim_hi && p.status) {
-          atomicOr(p.status, HC_ERR_RANGE);
-        }
-        meta[j & 3][lane] = mine;
-      }
+      blank(j, kr);
       store(smem + L::K + st * L::TILE, kr);
-      if (lane == 0) {                                  // after store()'s __syncwarp
-        if (w == 8) mbar_arrive(&bar.meta[j & 3]);
-        mbar_arrive(&bar.k_full[st]);
+      if (lane == 0) mbar_arrive(&bar.k_full[st]);      // after store()'s __syncwarp
+      if (j + 1 < n_tiles) {
+        load(p.kp, j + 1, kr);
+        lose();
       }
-      if (j + 1 < n_tiles) load(p.kp, j + 1, kr);
       if (j >= 2) ok = ok && wait_on(&bar.v_free[st], ((j >> 1) - 1) & 1);
       if (!__all_sync(0xffffffffu, ok)) break;
+      blank(j, vr);
       store(smem + L::V + st * L::TILE, vr);
       if (lane == 0) mbar_arrive(&bar.v_full[st]);
       if (j + 1 < n_tiles) {
         load(p.vp, j + 1, vr);
-        if (scales) {
-          at = next;
-          load_scales();
-        }
-        if (j + 2 < n_tiles) {
-          pages(j + 2);
-          if (scales) next = page_of(j + 2, lane);
-        }
+        lost = lost_next;
+        pages(j + 2);
       }
+    }
+  } else if (w == SCALE_WARP) {
+    // ---- scales: lane l has slice l of a tile; pages and scales run ahead ------
+    const int32_t* table = p.tables + (int64_t)r * p.t_stride;
+    const int key = (lane & (SLICES - 1)) * 16;
+    auto page_of = [&](int j) { return __ldg(table + (min(j * KT + key, lim_hi) >> p.page_log2)); };
+    auto head_of = [&](int page) { return (int64_t)((unsigned)page < (unsigned)p.n_pages ? page : 0) * p.nkv + h; };
+    int at = -1, next = -1;
+    float ks = 0.0f, vs = 1.0f;
+    if (n_tiles > 0) {
+      at = page_of(0);
+      next = page_of(1);
+      ks = __ldg(p.ks + head_of(at));
+      vs = __ldg(p.vs + head_of(at));
+    }
+    for (int j = 0; j < n_tiles; ++j) {
+      Slice mine = {0.0f, -INFINITY, 0.0f};             // no page: no weight
+      if ((unsigned)at < (unsigned)p.n_pages) {
+        const float b = fmaxf(vs, 1e-30f);
+        mine.k = ks;
+        mine.lv = __log2f(b);
+        mine.iv = __frcp_rn(b);
+      } else if (j * KT + key <= lim_hi && p.status) {
+        atomicOr(p.status, HC_ERR_RANGE);
+      }
+      if (j + 1 < n_tiles) {
+        at = next;
+        ks = __ldg(p.ks + head_of(at));
+        vs = __ldg(p.vs + head_of(at));
+        next = page_of(j + 2);
+      }
+      // the stage's keys are used up, so every reader of the slot is past it
+      if (j >= 2) ok = ok && wait_on(&bar.k_free[j & 1], ((j >> 1) - 1) & 1);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      if (lane < SLICES) meta[j & 3][lane] = mine;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar.meta[j & 3]);
     }
   } else if (n_tiles > 0) {
     // ---- MMA: one thread a group ----------------------------------------------
@@ -629,7 +668,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
         }
         mma_commit(&bar.s_full[g2][i & 1]);
       };
-      ok = wait_on(&bar.k_full[0], 0);
+      ok = wait_on(&bar.q_full[g2], 0) && wait_on(&bar.k_full[0], 0);
       if (ok) {
         fence_proxy();
         fence_after();
