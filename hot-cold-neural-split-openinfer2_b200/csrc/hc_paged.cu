@@ -285,16 +285,26 @@ struct Num<__nv_bfloat16> {
   static __device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __float2bfloat16_rn(x); }
 };
 
-// one output of a pair: x c + y s.  Queries in fp32 (one fma).  Keys in 64
-// bits, where both products are exact, then rounded to fp32 and to T: the
-// 16-bit value decides the byte that the cache holds, which then depends on no
-// order of operations.
-template <typename T, bool KEY>
+// x c + y s for one output of a pair.  Queries: one fma, rounded.
+template <typename T>
 __device__ __forceinline__ T turn(T x, T y, float c, float s) {
-  if constexpr (KEY)
-    return Num<T>::from_f((float)fma((double)Num<T>::to_f(y), (double)s, (double)Num<T>::to_f(x) * (double)c));
-  else
-    return Num<T>::from_f(fmaf(Num<T>::to_f(y), s, Num<T>::to_f(x) * c));
+  return Num<T>::from_f(fmaf(Num<T>::to_f(y), s, Num<T>::to_f(x) * c));
+}
+// Keys: the same to twice the precision (products split by fma, their sum by
+// two-sum), rounded to fp32 and then to T, which equals the 64-bit value
+// rounded so.  The 16-bit value decides the byte that the cache holds, which
+// then depends on no order of operations.  Conversions to 64 bits and back run
+// at a sixteenth of the fp32 rate here, so this costs half of what they do.
+__device__ __forceinline__ float turn_exact(float x, float y, float c, float s) {
+  const float p = __fmul_rn(x, c), q = __fmul_rn(y, s);
+  const float e = __fmaf_rn(x, c, -p), f = __fmaf_rn(y, s, -q);
+  const float r = __fadd_rn(p, q), z = __fsub_rn(r, p);
+  const float t = __fadd_rn(__fsub_rn(p, __fsub_rn(r, z)), __fsub_rn(q, z));
+  return __fadd_rn(r, __fadd_rn(t, __fadd_rn(e, f)));
+}
+template <typename T>
+__device__ __forceinline__ T turn_key(T x, T y, float c, float s) {
+  return Num<T>::from_f(turn_exact(Num<T>::to_f(x), Num<T>::to_f(y), c, s));
 }
 
 struct RopeArgs {
@@ -309,7 +319,7 @@ struct RopeArgs {
   const int64_t* positions;
   int n_rows, nq, nk, dim, rot;       // nk: key heads rotated by rope_rows (0 where they go into the cache)
   int interleaved;
-  int slots;                          // heads of one row worked on at once
+  int slots, rows_cta;                // heads of one row worked on at once; rows of a CTA (vector form)
   int32_t* status;
 };
 
@@ -324,83 +334,103 @@ __device__ __forceinline__ int64_t checked_pos(const int64_t* positions, int row
 
 // Vector form: a unit is 8 pairs (two 16-byte pieces of a head) or 16
 // elements that pass through.  A thread keeps its unit's 8 angles and walks
-// the row's heads with stride `slots`.  HBM-bound: each element read and
-// written once.
+// the row's heads with stride `slots`, four heads' loads in flight at a time.
+// HBM-bound: each element read and written once.
 template <typename T, bool KEY>
-__device__ __forceinline__ void rope_unit(const T* src, T* dst, int a0, int b0, bool turned, bool interleaved,
-                                          const float (&c)[8], const float (&s)[8]) {
+__device__ __forceinline__ void rope_unit(const uint4& av, const uint4& bv, T* dst, int a0, int b0, bool turned,
+                                          bool interleaved, const float (&c)[8], const float (&s)[8]) {
   __align__(16) T a[8], b[8], x[8], y[8];
-  *reinterpret_cast<uint4*>(a) = *reinterpret_cast<const uint4*>(src + a0);
-  *reinterpret_cast<uint4*>(b) = *reinterpret_cast<const uint4*>(src + b0);
+  *reinterpret_cast<uint4*>(a) = av;
+  *reinterpret_cast<uint4*>(b) = bv;
+  auto go = [](T u, T v, float cc, float ss) { return KEY ? turn_key<T>(u, v, cc, ss) : turn<T>(u, v, cc, ss); };
   if (!turned) {
-    *reinterpret_cast<uint4*>(dst + a0) = *reinterpret_cast<const uint4*>(a);
-    *reinterpret_cast<uint4*>(dst + b0) = *reinterpret_cast<const uint4*>(b);
+    *reinterpret_cast<uint4*>(dst + a0) = av;
+    *reinterpret_cast<uint4*>(dst + b0) = bv;
     return;
   }
   if (interleaved) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      x[2 * i] = turn<T, KEY>(a[2 * i], a[2 * i + 1], c[i], -s[i]);
-      x[2 * i + 1] = turn<T, KEY>(a[2 * i + 1], a[2 * i], c[i], s[i]);
-      y[2 * i] = turn<T, KEY>(b[2 * i], b[2 * i + 1], c[4 + i], -s[4 + i]);
-      y[2 * i + 1] = turn<T, KEY>(b[2 * i + 1], b[2 * i], c[4 + i], s[4 + i]);
+      x[2 * i] = go(a[2 * i], a[2 * i + 1], c[i], -s[i]);
+      x[2 * i + 1] = go(a[2 * i + 1], a[2 * i], c[i], s[i]);
+      y[2 * i] = go(b[2 * i], b[2 * i + 1], c[4 + i], -s[4 + i]);
+      y[2 * i + 1] = go(b[2 * i + 1], b[2 * i], c[4 + i], s[4 + i]);
     }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      x[i] = turn<T, KEY>(a[i], b[i], c[i], -s[i]);
-      y[i] = turn<T, KEY>(b[i], a[i], c[i], s[i]);
+      x[i] = go(a[i], b[i], c[i], -s[i]);
+      y[i] = go(b[i], a[i], c[i], s[i]);
     }
   }
   *reinterpret_cast<uint4*>(dst + a0) = *reinterpret_cast<const uint4*>(x);
   *reinterpret_cast<uint4*>(dst + b0) = *reinterpret_cast<const uint4*>(y);
 }
 
-template <typename T>
-__device__ __forceinline__ void rope_rows_vec(const RopeArgs& p, int64_t item0, int64_t items) {
-  const int units = p.dim / 16, heads = p.nq + p.nk;
-  const int64_t total = (int64_t)p.n_rows * p.slots * units;
-  for (int64_t it = item0; it < total; it += items) {
-    const int u = (int)(it % units), slot = (int)((it / units) % p.slots), row = (int)(it / units / p.slots);
-    const int64_t pos = checked_pos(p.positions, row, p.table_rows, p.status);
-    if (pos < 0) continue;
-    const bool turned = u < p.rot / 16;
-    float c[8], s[8];
+constexpr int BATCH = 4;                // heads of a thread in flight
+template <typename T, bool KEY>
+__device__ __forceinline__ void rope_heads(const T* src, int64_t src_head, T* dst, int64_t dst_head, int heads,
+                                           int slot, int slots, int a0, int b0, bool turned, bool interleaved,
+                                           const float (&c)[8], const float (&s)[8]) {
+  for (int h0 = slot; h0 < heads; h0 += BATCH * slots) {
+    uint4 a[BATCH], b[BATCH];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = s[i] = 0.0f;
-    if (turned) {
-      const float4* cr = reinterpret_cast<const float4*>(p.cos_t + pos * (p.rot / 2) + 8 * u);
-      const float4* sr = reinterpret_cast<const float4*>(p.sin_t + pos * (p.rot / 2) + 8 * u);
-      *reinterpret_cast<float4*>(c) = __ldg(cr);
-      *reinterpret_cast<float4*>(c + 4) = __ldg(cr + 1);
-      *reinterpret_cast<float4*>(s) = __ldg(sr);
-      *reinterpret_cast<float4*>(s + 4) = __ldg(sr + 1);
+    for (int k = 0; k < BATCH; ++k) {
+      const int h = min(h0 + k * slots, heads - 1);
+      a[k] = *reinterpret_cast<const uint4*>(src + h * src_head + a0);
+      b[k] = *reinterpret_cast<const uint4*>(src + h * src_head + b0);
     }
-    const bool pairs = p.interleaved || !turned;
-    const int a0 = pairs ? 16 * u : 8 * u, b0 = pairs ? 16 * u + 8 : p.rot / 2 + 8 * u;
-    for (int h = slot; h < heads; h += p.slots) {
-      if (h < p.nq) {
-        const T* src = static_cast<const T*>(p.q) + row * p.q_row + h * p.q_head;
-        T* dst = static_cast<T*>(p.q_out) + row * p.qo_row + h * p.qo_head;
-        if (turned || src != dst) rope_unit<T, false>(src, dst, a0, b0, turned, p.interleaved, c, s);
-      } else {
-        const T* src = static_cast<const T*>(p.k) + row * p.k_row + (h - p.nq) * p.k_head;
-        T* dst = static_cast<T*>(p.k_out) + row * p.ko_row + (h - p.nq) * p.ko_head;
-        if (turned || src != dst) rope_unit<T, true>(src, dst, a0, b0, turned, p.interleaved, c, s);
-      }
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      const int h = h0 + k * slots;
+      if (h < heads) rope_unit<T, KEY>(a[k], b[k], dst + h * dst_head, a0, b0, turned, interleaved, c, s);
     }
   }
 }
 
-// Any rotary size, stride and alignment: a thread per pair or passing element.
 template <typename T>
-__device__ __forceinline__ void rope_rows_any(const RopeArgs& p, int64_t item0, int64_t items) {
+__device__ __forceinline__ void rope_rows_vec(const RopeArgs& p, int block) {
+  const unsigned units = p.dim / 16, lanes = units * p.slots;
+  const unsigned in = threadIdx.x / lanes, rest = threadIdx.x - in * lanes;
+  const unsigned slot = rest / units, u = rest - slot * units;
+  const int64_t row = (int64_t)block * p.rows_cta + in;
+  if ((int)in >= p.rows_cta || row >= p.n_rows) return;
+  const int64_t pos = checked_pos(p.positions, row, p.table_rows, p.status);
+  if (pos < 0) return;
+  const bool turned = (int)u < p.rot / 16;
+  float c[8], s[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c[i] = s[i] = 0.0f;
+  if (turned) {
+    const float4* cr = reinterpret_cast<const float4*>(p.cos_t + pos * (p.rot / 2) + 8 * u);
+    const float4* sr = reinterpret_cast<const float4*>(p.sin_t + pos * (p.rot / 2) + 8 * u);
+    *reinterpret_cast<float4*>(c) = __ldg(cr);
+    *reinterpret_cast<float4*>(c + 4) = __ldg(cr + 1);
+    *reinterpret_cast<float4*>(s) = __ldg(sr);
+    *reinterpret_cast<float4*>(s + 4) = __ldg(sr + 1);
+  }
+  const bool pairs = p.interleaved || !turned;
+  const int a0 = pairs ? 16 * u : 8 * u, b0 = pairs ? 16 * u + 8 : p.rot / 2 + 8 * u;
+  const T* q = static_cast<const T*>(p.q) + row * p.q_row;
+  T* qo = static_cast<T*>(p.q_out) + row * p.qo_row;
+  if (turned || q != qo)
+    rope_heads<T, false>(q, p.q_head, qo, p.qo_head, p.nq, slot, p.slots, a0, b0, turned, p.interleaved, c, s);
+  const T* k = static_cast<const T*>(p.k) + row * p.k_row;
+  T* ko = static_cast<T*>(p.k_out) + row * p.ko_row;
+  if (p.nk && (turned || k != ko))
+    rope_heads<T, true>(k, p.k_head, ko, p.ko_head, p.nk, slot, p.slots, a0, b0, turned, p.interleaved, c, s);
+}
+
+// Any rotary size, stride and alignment: a row a CTA, a thread per pair or
+// passing element.
+template <typename T>
+__device__ __forceinline__ void rope_rows_any(const RopeArgs& p, int block) {
+  const int64_t row = block;
   const int half = p.rot / 2, units = half + p.dim - p.rot, heads = p.nq + p.nk;
-  const int64_t total = (int64_t)p.n_rows * heads * units;
-  for (int64_t it = item0; it < total; it += items) {
-    const int u = (int)(it % units), h = (int)((it / units) % heads), row = (int)(it / units / heads);
-    const int64_t pos = checked_pos(p.positions, row, p.table_rows, p.status);
-    if (pos < 0) continue;
+  const int64_t pos = checked_pos(p.positions, row, p.table_rows, p.status);
+  if (pos < 0) return;
+  for (unsigned it = threadIdx.x; it < (unsigned)(heads * units); it += blockDim.x) {
+    const int h = it / (unsigned)units, u = it - (unsigned)(h * units);
     const bool key = h >= p.nq;
     const T* src = key ? static_cast<const T*>(p.k) + row * p.k_row + (h - p.nq) * p.k_head
                        : static_cast<const T*>(p.q) + row * p.q_row + h * p.q_head;
@@ -413,8 +443,8 @@ __device__ __forceinline__ void rope_rows_any(const RopeArgs& p, int64_t item0, 
     const int i = p.interleaved ? 2 * u : u, j = p.interleaved ? 2 * u + 1 : u + half;
     const float c = __ldg(p.cos_t + pos * half + u), s = __ldg(p.sin_t + pos * half + u);
     const T a = src[i], b = src[j];
-    dst[i] = key ? turn<T, true>(a, b, c, -s) : turn<T, false>(a, b, c, -s);
-    dst[j] = key ? turn<T, true>(b, a, c, s) : turn<T, false>(b, a, c, s);
+    dst[i] = key ? turn_key<T>(a, b, c, -s) : turn<T>(a, b, c, -s);
+    dst[j] = key ? turn_key<T>(b, a, c, s) : turn<T>(b, a, c, s);
   }
 }
 
@@ -422,9 +452,8 @@ constexpr int ROPE_THREADS = 256;
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const RopeArgs p) {
-  const int64_t item0 = (int64_t)blockIdx.x * ROPE_THREADS + threadIdx.x, items = (int64_t)gridDim.x * ROPE_THREADS;
-  if constexpr (VEC) rope_rows_vec<T>(p, item0, items);
-  else rope_rows_any<T>(p, item0, items);
+  if constexpr (VEC) rope_rows_vec<T>(p, blockIdx.x);
+  else rope_rows_any<T>(p, blockIdx.x);
 }
 
 // ---------------------------------------------------------------------------
@@ -432,6 +461,8 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const RopeArgs p) {
 // ---------------------------------------------------------------------------
 constexpr int E_MIN = -40, E_MAX = 40;  // exponents of a page scale
 constexpr int CHUNK = 16;               // rows a warp holds at once
+constexpr int ANGLES = 2;
+constexpr int SPLIT_ROWS = 1024;        // rows from which the queries get a launch of their own
 constexpr int APPEND_THREADS = 256;
 constexpr int APPEND_WARPS = APPEND_THREADS / 32;
 
@@ -498,24 +529,87 @@ __device__ __forceinline__ void append_run(const AppendArgs& p, int which, int h
 #pragma unroll
       for (int e = 0; e < EL; ++e) x[e] = at[d0 + e];
     }
+  };
+  // the angles of this lane's elements (EL of them, or EL / 2 of neighbouring pairs)
+  const int half = ROPE ? p.rot / 2 : 0;
+  const bool second = ROPE && !p.interleaved && d0 >= half;
+  auto angles = [&](int64_t pos, float (&c)[EL], float (&s)[EL]) {
+    const int pair = p.interleaved ? d0 / 2 : second ? d0 - half : d0;
+    const float* cr = p.cos_t + pos * half + pair;
+    const float* sr = p.sin_t + pos * half + pair;
+    if (d0 >= p.rot) return;
+    if (p.interleaved) {
+#pragma unroll
+      for (int e = 0; e < EL / 2; ++e) c[e] = __ldg(cr + e), s[e] = __ldg(sr + e);
+    } else if constexpr (EL == 4) {
+      *reinterpret_cast<float4*>(c) = __ldg(reinterpret_cast<const float4*>(cr));
+      *reinterpret_cast<float4*>(s) = __ldg(reinterpret_cast<const float4*>(sr));
+    } else {
+      *reinterpret_cast<float2*>(c) = __ldg(reinterpret_cast<const float2*>(cr));
+      *reinterpret_cast<float2*>(s) = __ldg(reinterpret_cast<const float2*>(sr));
+    }
+  };
+  // rotates a row that load() brought; every lane of the warp takes part.  The
+  // other halves of its pairs are in this lane, or `half` elements away in another.
+  auto rotate = [&](const float (&c)[EL], const float (&s)[EL], T (&x)[EL]) {
+    T o[EL];
+    if (!p.interleaved) {
+      const int from = second ? lane - half / EL : lane + half / EL;
+      if constexpr (EL == 4) {
+        const uint2 v = *reinterpret_cast<const uint2*>(x);
+        *reinterpret_cast<uint2*>(o) =
+            make_uint2(__shfl_sync(0xffffffffu, v.x, from & 31), __shfl_sync(0xffffffffu, v.y, from & 31));
+      } else {
+        *reinterpret_cast<uint32_t*>(o) = __shfl_sync(0xffffffffu, *reinterpret_cast<const uint32_t*>(x), from & 31);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < EL; ++e) o[e] = x[e ^ 1];
+    }
+    if (d0 >= p.rot) return;
+#pragma unroll
+    for (int e = 0; e < EL; ++e) {
+      const float cc = p.interleaved ? c[e / 2] : c[e], ss = p.interleaved ? s[e / 2] : s[e];
+      x[e] = turn_key<T>(x[e], o[e], cc, (p.interleaved ? (e & 1) : second) ? ss : -ss);
+    }
+  };
+  // the same for any rotary size and alignment
+  auto rotate_any = [&](int row, int64_t pos, T (&x)[EL]) {
+    const T* at = src + row * step;
+#pragma unroll
+    for (int e = 0; e < EL; ++e) {
+      const int d = d0 + e;
+      if (d >= p.rot) continue;
+      const bool sec = p.interleaved ? (d & 1) : d >= half;
+      const int pair = p.interleaved ? d >> 1 : sec ? d - half : d;
+      const T mine = at[d], other = at[p.interleaved ? d ^ 1 : sec ? d - half : d + half];
+      const float c = __ldg(p.cos_t + pos * half + pair), s = __ldg(p.sin_t + pos * half + pair);
+      x[e] = turn_key<T>(mine, other, c, sec ? s : -s);
+    }
+  };
+  // up to CHUNK rows from row0 + j0 on, all loads in flight before the first is used
+  auto load_chunk = [&](int j0, T (&x)[CHUNK][EL]) {
+#pragma unroll
+    for (int j = 0; j < CHUNK; ++j)
+      if (j0 + j < n) load(row0 + j0 + j, x[j]);
     if constexpr (ROPE) {
       if (which == 0) {
-        const int64_t pos = p.positions[row];
-        const int half = p.rot / 2;
-        T y[EL];
+        const int64_t mine = p.positions[row0 + min(j0 + (lane & (CHUNK - 1)), n - 1)];
+        if constexpr (VEC) {
 #pragma unroll
-        for (int e = 0; e < EL; ++e) {
-          const int d = d0 + e;
-          y[e] = x[e];
-          if (d >= p.rot) continue;
-          const bool second = p.interleaved ? (d & 1) : d >= half;
-          const int pair = p.interleaved ? d >> 1 : second ? d - half : d;
-          const T other = at[p.interleaved ? d ^ 1 : second ? d - half : d + half];
-          const float c = __ldg(p.cos_t + pos * half + pair), s = __ldg(p.sin_t + pos * half + pair);
-          y[e] = turn<T, true>(x[e], other, c, second ? s : -s);
+          for (int j = 0; j < CHUNK; j += ANGLES) {    // ANGLES rows' angles in flight
+            if (j0 + j >= n) break;
+            float c[ANGLES][EL], s[ANGLES][EL];
+#pragma unroll
+            for (int e = 0; e < ANGLES; ++e) angles(__shfl_sync(0xffffffffu, mine, j + e), c[e], s[e]);
+#pragma unroll
+            for (int e = 0; e < ANGLES; ++e) rotate(c[e], s[e], x[j + e]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < CHUNK; ++j)
+            if (j0 + j < n) rotate_any(row0 + j0 + j, __shfl_sync(0xffffffffu, mine, j), x[j]);
         }
-#pragma unroll
-        for (int e = 0; e < EL; ++e) x[e] = y[e];
       }
     }
   };
@@ -525,9 +619,7 @@ __device__ __forceinline__ void append_run(const AppendArgs& p, int which, int h
   float top = 0.0f;
   bool odd = false;
   for (int j0 = 0; j0 < n; j0 += CHUNK) {
-#pragma unroll
-    for (int j = 0; j < CHUNK; ++j)
-      if (j0 + j < n) load(row0 + j0 + j, x[j]);
+    load_chunk(j0, x);
 #pragma unroll
     for (int j = 0; j < CHUNK; ++j)
       if (j0 + j < n) {
@@ -567,11 +659,7 @@ __device__ __forceinline__ void append_run(const AppendArgs& p, int which, int h
   if (lane == 0 && (grown || !lo)) *scale_at = now;
 
   for (int j0 = 0; j0 < n; j0 += CHUNK) {
-    if (n > CHUNK) {
-#pragma unroll
-      for (int j = 0; j < CHUNK; ++j)
-        if (j0 + j < n) load(row0 + j0 + j, x[j]);
-    }
+    if (n > CHUNK) load_chunk(j0, x);
 #pragma unroll
     for (int j = 0; j < CHUNK; ++j)
       if (j0 + j < n) {
@@ -636,21 +724,22 @@ __device__ __forceinline__ void append_rows(const AppendArgs& p, int t0, int t1,
   }
 }
 
-// Blocks below `n_append` write the cache, the others rotate the queries.
+// n_append blocks write the cache, the others rotate the queries; the two kinds
+// alternate over the grid, since one is bound by latency and the other by HBM.
 template <typename T, int EL, bool VEC, bool ROPE>
-__global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendArgs p, const RopeArgs rope, int n_append,
-                                                                int groups) {
-  if ((int)blockIdx.x < n_append) {
-    const int item = (int)(blockIdx.x % groups) * APPEND_WARPS + (threadIdx.x >> 5);
-    const int t0 = (int)(blockIdx.x / groups) * p.seg;
+__global__ void __launch_bounds__(APPEND_THREADS, 2) append_kernel(const AppendArgs p, const RopeArgs rope,
+                                                                unsigned n_append, unsigned groups) {
+  const unsigned before = (unsigned)((uint64_t)blockIdx.x * n_append / gridDim.x);
+  const unsigned upto = (unsigned)((uint64_t)(blockIdx.x + 1) * n_append / gridDim.x);
+  if (upto > before) {
+    const int item = (int)(before % groups) * APPEND_WARPS + (threadIdx.x >> 5);
+    const int t0 = (int)(before / groups) * p.seg;
     if (item < 2 * p.n_kv) append_rows<T, EL, VEC, ROPE>(p, t0, min(p.n_rows, t0 + p.seg), item);
     return;
   }
   if constexpr (ROPE) {
-    const int64_t item0 = (int64_t)(blockIdx.x - n_append) * APPEND_THREADS + threadIdx.x;
-    const int64_t items = (int64_t)(gridDim.x - n_append) * APPEND_THREADS;
-    if constexpr (VEC) rope_rows_vec<T>(rope, item0, items);
-    else rope_rows_any<T>(rope, item0, items);
+    if constexpr (VEC) rope_rows_vec<T>(rope, blockIdx.x - before);
+    else rope_rows_any<T>(rope, blockIdx.x - before);
   }
 }
 
@@ -676,7 +765,7 @@ int check_rope(const hc_rope_args* a, bool to_cache) {
 
 // The vector form wants 16-byte pieces throughout and whole units of 8 pairs.
 bool rope_vec(const hc_rope_args* a, bool keys) {
-  bool ok = multiple(a->rotary_dim, 16) && multiple(a->head_dim, 16) && aligned(a->q, 16) && aligned(a->q_out, 16) &&
+  bool ok = multiple(a->rotary_dim, 16) && multiple(a->head_dim, 16) && a->head_dim <= 16 * ROPE_THREADS && aligned(a->q, 16) && aligned(a->q_out, 16) &&
             multiple(a->q_row, 8) && multiple(a->q_head, 8) && multiple(a->q_out_row, 8) &&
             multiple(a->q_out_head, 8) && aligned(a->cos_t, 16) && aligned(a->sin_t, 16);
   if (keys)
@@ -715,18 +804,16 @@ RopeArgs rope_args(const hc_rope_args* a, bool keys, int32_t* status) {
 }
 
 // Blocks of the rotation; sets how many heads of a row are worked on at once:
-// all of them while rows are few, a fifth when they fill the GPU anyway.
-int rope_blocks(RopeArgs& p, bool vec) {
-  const int heads = p.nq + p.nk;
-  int64_t threads;
-  if (vec) {
-    const int units = p.dim / 16;
-    p.slots = (int64_t)p.n_rows * units * heads <= 148 * 2048 ? heads : (heads + 4) / 5;
-    threads = (int64_t)p.n_rows * units * p.slots;
-  } else {
-    threads = (int64_t)p.n_rows * heads * (p.dim - p.rot / 2);
-  }
-  return (int)min((threads + ROPE_THREADS - 1) / ROPE_THREADS, (int64_t)148 * 64);
+// all that a block has room for while rows are few, a quarter of them (each
+// thread then has four heads' loads in flight) when rows fill the GPU.
+int64_t rope_blocks(RopeArgs& p, bool vec) {
+  p.rows_cta = 1;
+  if (!vec) return p.n_rows;
+  const int units = p.dim / 16, room = max(1, ROPE_THREADS / units);
+  p.slots = min(room, max(p.nq, p.nk));
+  if ((int64_t)p.n_rows * units * p.slots > 148 * 2048) p.slots = min(room, (max(p.nq, p.nk) + BATCH - 1) / BATCH);
+  p.rows_cta = max(1, ROPE_THREADS / (units * p.slots));
+  return (p.n_rows + p.rows_cta - 1) / p.rows_cta;
 }
 
 int check_pages(const hc_kv_pages* c) {
@@ -743,7 +830,7 @@ int check_pages(const hc_kv_pages* c) {
 template <typename T>
 int launch_append(AppendArgs& p, const hc_rope_args* rope, const hc_kv_pages* c, cudaStream_t stream) {
   RopeArgs ra = {};
-  int extra = 0;
+  int64_t extra = 0;
   const int align = c->head_dim == 128 ? 4 : 2;      // elements a lane loads at once
   bool vec = aligned(p.src[0], 2 * align) && aligned(p.src[1], 2 * align) && multiple(p.src_row[0], align) &&
              multiple(p.src_row[1], align) && multiple(p.src_head[0], align) && multiple(p.src_head[1], align);
@@ -756,9 +843,17 @@ int launch_append(AppendArgs& p, const hc_rope_args* rope, const hc_kv_pages* c,
   p.seg = max(1, min(32, p.n_rows / 256));
   const int groups = (2 * p.n_kv + APPEND_WARPS - 1) / APPEND_WARPS;
   const int64_t n_append = (int64_t)((p.n_rows + p.seg - 1) / p.seg) * groups;
+  // Few rows: one launch does both.  Many: the queries' rotation needs half of the registers that the write
+  // does, and runs faster as a kernel of its own.
+  const bool together = p.n_rows < SPLIT_ROWS;
+  if (rope && !together && extra > 0) {
+    if (vec) rope_kernel<T, true><<<(unsigned)extra, ROPE_THREADS, 0, stream>>>(ra);
+    else rope_kernel<T, false><<<(unsigned)extra, ROPE_THREADS, 0, stream>>>(ra);
+    extra = 0;
+  }
   if (n_append + extra > INT32_MAX) return HC_ERR_UNSUPPORTED;
   const dim3 grid((unsigned)(n_append + extra));
-#define GO(EL, V, R) append_kernel<T, EL, V, R><<<grid, APPEND_THREADS, 0, stream>>>(p, ra, (int)n_append, groups)
+#define GO(EL, V, R) append_kernel<T, EL, V, R><<<grid, APPEND_THREADS, 0, stream>>>(p, ra, (unsigned)n_append, (unsigned)groups)
   if (c->head_dim == 128) {
     if (rope) {
       if (vec) GO(4, true, true);
@@ -851,7 +946,7 @@ extern "C" int hc_rope(const hc_rope_args* a, int32_t* status, hc_stream_t strea
   if (a->n_rows == 0) return HC_OK;
   const bool vec = rope_vec(a, true);
   RopeArgs p = rope_args(a, true, status);
-  const int blocks = rope_blocks(p, vec);
+  const int blocks = (int)rope_blocks(p, vec);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (a->dtype == HC_F16) {
     if (vec) rope_kernel<__half, true><<<blocks, ROPE_THREADS, 0, s>>>(p);

@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
       auto scores = [&](int i) {
         uint64_t a = d_q, b = d_k + place(i);
         const uint32_t d = t_s + HALF * (i & 1);
-#pragma unroll 1
+#pragma unroll
         for (int e = 0; e < D / 64; ++e) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) mma_ss(d, a + 2 * k, b + 2 * k, id_s, e + k);
