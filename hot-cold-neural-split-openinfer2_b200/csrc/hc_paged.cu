@@ -452,6 +452,7 @@ constexpr int ROPE_THREADS = 256;
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const RopeArgs p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if constexpr (VEC) rope_rows_vec<T>(p, blockIdx.x);
   else rope_rows_any<T>(p, blockIdx.x);
 }
@@ -461,7 +462,6 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const RopeArgs p) {
 // ---------------------------------------------------------------------------
 constexpr int E_MIN = -40, E_MAX = 40;  // exponents of a page scale
 constexpr int CHUNK = 16;               // rows a warp holds at once
-constexpr int ANGLES = 2;
 constexpr int SPLIT_ROWS = 1024;        // rows from which the queries get a launch of their own
 constexpr int APPEND_THREADS = 256;
 constexpr int APPEND_WARPS = APPEND_THREADS / 32;
@@ -475,6 +475,8 @@ struct AppendArgs {
   const int64_t* slots;
   int n_rows;
   int seg;                            // rows a CTA looks for runs in
+  int wpi;                            // warps of an item (one head's keys or values of a run)
+  int beside;                         // runs beside the queries' kernel
   // rotation of the keys (fused form)
   const float* cos_t;
   const float* sin_t;
@@ -502,13 +504,15 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   return r;
 }
 
-// One warp writes one run (the consecutive rows that enter one page) of one
-// head's keys or values.  EL elements of a row per lane; the run's rows are
-// held 16 at a time, and read again when the run is longer (its largest
-// value has to be known first).  Latency-bound for decode (one row a run),
-// HBM-bound for prompts.
+// Writes one run (the consecutive rows that enter one page) of one head's keys
+// or values: `wpi` warps, each with 16 rows in registers (EL elements of a row
+// per lane), so a run of up to 16 wpi rows is read once and a longer one twice;
+// the warps' largest values meet in shared memory.  The angles of a warp's rows
+// come through shared memory, all copies in flight at once.  Latency-bound.
+// Every warp of the block calls it for the same run (`idle`: without an item).
 template <typename T, int EL, bool VEC, bool ROPE>
-__device__ __forceinline__ void append_run(const AppendArgs& p, int which, int head, int row0, int n, int64_t slot0) {
+__device__ __forceinline__ void append_run(const AppendArgs& p, int which, int head, int wi, bool idle, float* s_top,
+                                           float* angles, int row0, int n, int64_t slot0) {
   constexpr int D = 32 * EL;
   const int lane = threadIdx.x & 31;
   const int64_t page = slot0 >> p.page_log2;
@@ -517,8 +521,9 @@ __device__ __forceinline__ void append_run(const AppendArgs& p, int which, int h
   float* scale_at = p.scales[which] + page * p.n_kv + head;
   const T* src = static_cast<const T*>(p.src[which]) + head * p.src_head[which];
   const int64_t step = p.src_row[which];
-  const float old = lo ? *scale_at : 0.0f;           // a run from the page's first row begins the page anew
-  const int d0 = EL * lane;
+  const float old = lo && !idle ? *scale_at : 0.0f;  // a run from the page's first row begins the page anew
+  const int d0 = EL * lane, span = CHUNK * p.wpi;
+  if (idle) n = 0;
 
   auto load = [&](int row, T (&x)[EL]) {
     const T* at = src + row * step;
@@ -530,28 +535,12 @@ __device__ __forceinline__ void append_run(const AppendArgs& p, int which, int h
       for (int e = 0; e < EL; ++e) x[e] = at[d0 + e];
     }
   };
-  // the angles of this lane's elements (EL of them, or EL / 2 of neighbouring pairs)
   const int half = ROPE ? p.rot / 2 : 0;
   const bool second = ROPE && !p.interleaved && d0 >= half;
-  auto angles = [&](int64_t pos, float (&c)[EL], float (&s)[EL]) {
-    const int pair = p.interleaved ? d0 / 2 : second ? d0 - half : d0;
-    const float* cr = p.cos_t + pos * half + pair;
-    const float* sr = p.sin_t + pos * half + pair;
-    if (d0 >= p.rot) return;
-    if (p.interleaved) {
-#pragma unroll
-      for (int e = 0; e < EL / 2; ++e) c[e] = __ldg(cr + e), s[e] = __ldg(sr + e);
-    } else if constexpr (EL == 4) {
-      *reinterpret_cast<float4*>(c) = __ldg(reinterpret_cast<const float4*>(cr));
-      *reinterpret_cast<float4*>(s) = __ldg(reinterpret_cast<const float4*>(sr));
-    } else {
-      *reinterpret_cast<float2*>(c) = __ldg(reinterpret_cast<const float2*>(cr));
-      *reinterpret_cast<float2*>(s) = __ldg(reinterpret_cast<const float2*>(sr));
-    }
-  };
-  // rotates a row that load() brought; every lane of the warp takes part.  The
-  // other halves of its pairs are in this lane, or `half` elements away in another.
-  auto rotate = [&](const float (&c)[EL], const float (&s)[EL], T (&x)[EL]) {
+  // rotates a row that load() brought by the angles at `c` and c + half; every
+  // lane of the warp takes part.  The other halves of its pairs are in this
+  // lane, or `half` elements away in another.
+  auto rotate = [&](const float* c, T (&x)[EL]) {
     T o[EL];
     if (!p.interleaved) {
       const int from = second ? lane - half / EL : lane + half / EL;
@@ -562,15 +551,17 @@ __device__ __forceinline__ void append_run(const AppendArgs& p, int which, int h
       } else {
         *reinterpret_cast<uint32_t*>(o) = __shfl_sync(0xffffffffu, *reinterpret_cast<const uint32_t*>(x), from & 31);
       }
+      if (d0 >= p.rot) return;
+      c += second ? d0 - half : d0;
+#pragma unroll
+      for (int e = 0; e < EL; ++e) x[e] = turn_key<T>(x[e], o[e], c[e], second ? c[half + e] : -c[half + e]);
     } else {
+      if (d0 >= p.rot) return;
+      c += d0 / 2;
 #pragma unroll
-      for (int e = 0; e < EL; ++e) o[e] = x[e ^ 1];
-    }
-    if (d0 >= p.rot) return;
+      for (int e = 0; e < EL; ++e) o[e] = x[e];
 #pragma unroll
-    for (int e = 0; e < EL; ++e) {
-      const float cc = p.interleaved ? c[e / 2] : c[e], ss = p.interleaved ? s[e / 2] : s[e];
-      x[e] = turn_key<T>(x[e], o[e], cc, (p.interleaved ? (e & 1) : second) ? ss : -ss);
+      for (int e = 0; e < EL; ++e) x[e] = turn_key<T>(o[e], o[e ^ 1], c[e / 2], e & 1 ? c[half + e / 2] : -c[half + e / 2]);
     }
   };
   // the same for any rotary size and alignment
@@ -587,39 +578,53 @@ __device__ __forceinline__ void append_run(const AppendArgs& p, int which, int h
       x[e] = turn_key<T>(mine, other, c, sec ? s : -s);
     }
   };
-  // up to CHUNK rows from row0 + j0 on, all loads in flight before the first is used
-  auto load_chunk = [&](int j0, T (&x)[CHUNK][EL]) {
-#pragma unroll
-    for (int j = 0; j < CHUNK; ++j)
-      if (j0 + j < n) load(row0 + j0 + j, x[j]);
+  // rows j0 .. of the run, all loads in flight before the first is used
+  T x[CHUNK][EL];
+  auto load_chunk = [&](int j0) {
+    const int m = n - j0, row = row0 + j0;
+    int64_t pos = 0;
     if constexpr (ROPE) {
       if (which == 0) {
-        const int64_t mine = p.positions[row0 + min(j0 + (lane & (CHUNK - 1)), n - 1)];
-        if constexpr (VEC) {
+        pos = p.positions[row + min(lane & (CHUNK - 1), m - 1)];
+        if constexpr (VEC) {                           // lane l copies piece l of a row's cosines and sines
+          const bool sine = 4 * lane >= half;
+          const float* table = sine ? p.sin_t + 4 * lane - half : p.cos_t + 4 * lane;
+          const uint32_t to = smem_u32(angles) + 16 * lane;
 #pragma unroll
-          for (int j = 0; j < CHUNK; j += ANGLES) {    // ANGLES rows' angles in flight
-            if (j0 + j >= n) break;
-            float c[ANGLES][EL], s[ANGLES][EL];
-#pragma unroll
-            for (int e = 0; e < ANGLES; ++e) angles(__shfl_sync(0xffffffffu, mine, j + e), c[e], s[e]);
-#pragma unroll
-            for (int e = 0; e < ANGLES; ++e) rotate(c[e], s[e], x[j + e]);
+          for (int j = 0; j < CHUNK; ++j) {
+            const int64_t at = __shfl_sync(0xffffffffu, pos, j);
+            if (j < m && 2 * lane < half)
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(to + j * D * 4), "l"(table + at * half)
+                           : "memory");
           }
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < CHUNK; ++j)
+      if (j < m) load(row + j, x[j]);
+    if constexpr (ROPE) {
+      if (which == 0) {
+        if constexpr (VEC) {
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < CHUNK; ++j)
+            if (j < m) rotate(angles + j * D, x[j]);
+          __syncwarp();
         } else {
 #pragma unroll
           for (int j = 0; j < CHUNK; ++j)
-            if (j0 + j < n) rotate_any(row0 + j0 + j, __shfl_sync(0xffffffffu, mine, j), x[j]);
+            if (j < m) rotate_any(row + j, __shfl_sync(0xffffffffu, pos, j), x[j]);
         }
       }
     }
   };
-
   // largest finite value of the run
-  T x[CHUNK][EL];
   float top = 0.0f;
   bool odd = false;
-  for (int j0 = 0; j0 < n; j0 += CHUNK) {
-    load_chunk(j0, x);
+  for (int j0 = CHUNK * wi; j0 < n; j0 += span) {
+    load_chunk(j0);
 #pragma unroll
     for (int j = 0; j < CHUNK; ++j)
       if (j0 + j < n) {
@@ -634,6 +639,11 @@ __device__ __forceinline__ void append_run(const AppendArgs& p, int which, int h
   if (__any_sync(0xffffffffu, odd) && lane == 0 && p.status) atomicOr(p.status, HC_ERR_RANGE);
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) s_top[threadIdx.x >> 5] = top;
+  __syncthreads();                                   // also: every warp has read the old scale
+  if (idle) return;
+  const int w0 = (int)(threadIdx.x >> 5) - wi;       // the item's first warp
+  for (int k = 0; k < p.wpi; ++k) top = fmaxf(top, s_top[w0 + k]);
   const float need = pow2f(scale_exponent(top));
   const bool grown = need > old;
   const float now = grown ? need : old;
@@ -642,7 +652,7 @@ __device__ __forceinline__ void append_run(const AppendArgs& p, int which, int h
   // the page's older rows at the larger scale
   if (lo && grown) {
     const float f = old * inv;
-    for (int i = lane; i < lo * D / 16; i += 32) {
+    for (int i = 32 * wi + lane; i < lo * D / 16; i += 32 * p.wpi) {
       uint4* at = reinterpret_cast<uint4*>(dst) + i;
       uint4 w = *at;
       uint32_t* ws = reinterpret_cast<uint32_t*>(&w);
@@ -656,10 +666,9 @@ __device__ __forceinline__ void append_run(const AppendArgs& p, int which, int h
       *at = w;
     }
   }
-  if (lane == 0 && (grown || !lo)) *scale_at = now;
-
-  for (int j0 = 0; j0 < n; j0 += CHUNK) {
-    if (n > CHUNK) load_chunk(j0, x);
+  if (wi == 0 && lane == 0 && (grown || !lo)) *scale_at = now;
+  for (int j0 = CHUNK * wi; j0 < n; j0 += span) {
+    if (n > span) load_chunk(j0);
 #pragma unroll
     for (int j = 0; j < CHUNK; ++j)
       if (j0 + j < n) {
@@ -694,20 +703,24 @@ __device__ __forceinline__ int64_t checked_slot(const AppendArgs& p, int t, bool
 
 // Runs that begin among rows [t0, t1), t1 - t0 <= 32: a row begins one unless
 // the row before it lies in the same page.  Rows of a page that do not follow
-// one another are flagged and left out.
+// one another are flagged and left out.  The whole block works on one run.
 template <typename T, int EL, bool VEC, bool ROPE>
-__device__ __forceinline__ void append_rows(const AppendArgs& p, int t0, int t1, int item) {
-  const int lane = threadIdx.x & 31, which = item & 1, head = item >> 1;
+__device__ __forceinline__ void append_rows(const AppendArgs& p, int t0, int t1, int item, int wi,
+                                            float (*s_top)[APPEND_WARPS], float* angles) {
+  const int lane = threadIdx.x & 31, which = item & 1;
+  const bool idle = item >= 2 * p.n_kv, flag = item == 0 && wi == 0;
+  const int head = idle ? 0 : item >> 1;
   const int mine = t0 + lane;
   int64_t slot = -1;
   bool begins = false;
   if (mine < t1) {
-    slot = checked_slot<ROPE>(p, mine, item == 0);
+    slot = checked_slot<ROPE>(p, mine, flag);
     const int64_t before = mine ? checked_slot<ROPE>(p, mine - 1, false) : -1;
     const bool same = slot >= 0 && before >= 0 && before >> p.page_log2 == slot >> p.page_log2;
     begins = slot >= 0 && !same;
-    if (same && before + 1 != slot && item == 0 && p.status) atomicOr(p.status, HC_ERR_RANGE);
+    if (same && before + 1 != slot && flag && p.status) atomicOr(p.status, HC_ERR_RANGE);
   }
+  int turn = 0;
   for (uint32_t todo = __ballot_sync(0xffffffffu, begins); todo; todo &= todo - 1) {
     const int from = __ffs(todo) - 1, t = t0 + from;
     const int64_t first = __shfl_sync(0xffffffffu, slot, from);
@@ -720,7 +733,7 @@ __device__ __forceinline__ void append_rows(const AppendArgs& p, int t0, int t1,
       n += ok == 0xffffffffu ? 32 : __ffs(~ok) - 1;
       if (ok != 0xffffffffu) break;
     }
-    append_run<T, EL, VEC, ROPE>(p, which, head, t, n, first);
+    append_run<T, EL, VEC, ROPE>(p, which, head, wi, idle, s_top[turn ^= 1], angles, t, n, first);
   }
 }
 
@@ -732,9 +745,14 @@ __global__ void __launch_bounds__(APPEND_THREADS, 2) append_kernel(const AppendA
   const unsigned before = (unsigned)((uint64_t)blockIdx.x * n_append / gridDim.x);
   const unsigned upto = (unsigned)((uint64_t)(blockIdx.x + 1) * n_append / gridDim.x);
   if (upto > before) {
-    const int item = (int)(before % groups) * APPEND_WARPS + (threadIdx.x >> 5);
+    extern __shared__ __align__(16) float s_angles[];                // [warp][CHUNK][dim]
+    __shared__ float s_top[2][APPEND_WARPS];
+    const int w = threadIdx.x >> 5;
+    const int item = (int)(before % groups) * (APPEND_WARPS / p.wpi) + w / p.wpi;
     const int t0 = (int)(before / groups) * p.seg;
-    if (item < 2 * p.n_kv) append_rows<T, EL, VEC, ROPE>(p, t0, min(p.n_rows, t0 + p.seg), item);
+    append_rows<T, EL, VEC, ROPE>(p, t0, min(p.n_rows, t0 + p.seg), item, w % p.wpi, s_top,
+                                  s_angles + w * CHUNK * 32 * EL);
+    if (p.beside) asm volatile("griddepcontrol.wait;" ::: "memory");   // the queries' kernel ends no later than this
     return;
   }
   if constexpr (ROPE) {
@@ -839,40 +857,59 @@ int launch_append(AppendArgs& p, const hc_rope_args* rope, const hc_kv_pages* c,
     ra = rope_args(rope, false, p.status);
     extra = rope_blocks(ra, vec);
   }
-  // rows a CTA searches: one while rows are few (decode: every row is a run), more for prompts
-  p.seg = max(1, min(32, p.n_rows / 256));
-  const int groups = (2 * p.n_kv + APPEND_WARPS - 1) / APPEND_WARPS;
+  // Rows a CTA searches: one while rows are few (decode: every row is a run), about a page for prompts.
+  p.seg = max(1, min(min(32, c->page_size), p.n_rows / 256));
+  // Warps of an item: enough to hold a whole page when rows are many; with few, most runs are single rows and
+  // more warps only wait.
+  p.wpi = min(c->page_size / CHUNK, p.n_rows <= 256 ? 1 : p.n_rows < SPLIT_ROWS ? 2 : 8);
+  const int items = APPEND_WARPS / p.wpi;
+  const int groups = (2 * p.n_kv + items - 1) / items;
   const int64_t n_append = (int64_t)((p.n_rows + p.seg - 1) / p.seg) * groups;
   // Few rows: one launch does both.  Many: the queries' rotation needs half of the registers that the write
-  // does, and runs faster as a kernel of its own.
-  const bool together = p.n_rows < SPLIT_ROWS;
-  if (rope && !together && extra > 0) {
+  // does, and runs faster as a kernel of its own, which the write may run beside.
+  if (rope && p.n_rows >= SPLIT_ROWS) {
     if (vec) rope_kernel<T, true><<<(unsigned)extra, ROPE_THREADS, 0, stream>>>(ra);
     else rope_kernel<T, false><<<(unsigned)extra, ROPE_THREADS, 0, stream>>>(ra);
+    if (cudaGetLastError() != cudaSuccess) return HC_ERR_CUDA;
     extra = 0;
+    p.beside = 1;
   }
   if (n_append + extra > INT32_MAX) return HC_ERR_UNSUPPORTED;
-  const dim3 grid((unsigned)(n_append + extra));
-#define GO(EL, V, R) append_kernel<T, EL, V, R><<<grid, APPEND_THREADS, 0, stream>>>(p, ra, (unsigned)n_append, (unsigned)groups)
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(n_append + extra));
+  cfg.blockDim = dim3(APPEND_THREADS);
+  cfg.dynamicSmemBytes = rope && vec ? APPEND_WARPS * CHUNK * c->head_dim * 4 : 0;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = p.beside ? 1 : 0;
+  cudaError_t rc;
+#define GO(EL, V, R)                                                                                          \
+  rc = R && V ? cudaFuncSetAttribute(append_kernel<T, EL, V, R>, cudaFuncAttributeMaxDynamicSharedMemorySize,  \
+                                     (int)cfg.dynamicSmemBytes)                                               \
+              : cudaSuccess;                                                                                  \
+  if (rc == cudaSuccess) rc = cudaLaunchKernelEx(&cfg, append_kernel<T, EL, V, R>, p, ra, (unsigned)n_append, (unsigned)groups)
   if (c->head_dim == 128) {
     if (rope) {
-      if (vec) GO(4, true, true);
-      else GO(4, false, true);
+      if (vec) { GO(4, true, true); }
+      else { GO(4, false, true); }
     } else {
-      if (vec) GO(4, true, false);
-      else GO(4, false, false);
+      if (vec) { GO(4, true, false); }
+      else { GO(4, false, false); }
     }
   } else {
     if (rope) {
-      if (vec) GO(2, true, true);
-      else GO(2, false, true);
+      if (vec) { GO(2, true, true); }
+      else { GO(2, false, true); }
     } else {
-      if (vec) GO(2, true, false);
-      else GO(2, false, false);
+      if (vec) { GO(2, true, false); }
+      else { GO(2, false, false); }
     }
   }
 #undef GO
-  return cudaGetLastError() == cudaSuccess ? HC_OK : HC_ERR_CUDA;
+  return rc == cudaSuccess ? HC_OK : HC_ERR_CUDA;
 }
 
 AppendArgs append_args(const hc_kv_pages* c, const void* k, int64_t k_row, int64_t k_head, const void* v,
