@@ -626,6 +626,7 @@ extern "C" int hc_paged_attn(const hc_attn_args* a, const hc_kv_pages* c, void* 
       a->n_q_heads % c->n_kv_heads || a->table_width <= 0 || a->table_stride < a->table_width ||
       (a->dtype != HC_F16 && a->dtype != HC_BF16))
     return HC_ERR_ARG;
+  if (a->q_row < 0 || a->q_head < 0 || a->out_row < 0 || a->out_head < 0) return HC_ERR_ARG;
   if (!aligned(a->q, 2) || !aligned(a->out, 2) || !aligned(a->lse, 4) || !aligned(c->k, 16) || !aligned(c->v, 16) ||
       !aligned(a->tables, 4) || !aligned(c->k_scale, 4) || !aligned(c->v_scale, 4))
     return HC_ERR_ARG;

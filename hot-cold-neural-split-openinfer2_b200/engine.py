@@ -22,12 +22,14 @@ import math
 from pathlib import Path
 from typing import Optional, Sequence
 
+import numpy as np
 import torch
 import torch.distributed
 import torch.nn as nn
 import torch.nn.functional as F
 
 import hc_native as N
+import paged
 from predictor import NeuronPredictor, PredictorRegistry, logit_threshold, unpack_mask
 from splitter import HIDDEN_DIM, NEURON_RECORD_BYTES, ColdWeightStore, bits_to_words
 
@@ -919,6 +921,10 @@ class GroupedQueryAttention(nn.Module):
             w8 = lambda n: weights[pre + n].to(dev).to(torch.float8_e4m3fn).view(torch.uint8)
             self.qkv_w8 = torch.cat([w8("q_proj"), w8("k_proj"), w8("v_proj")], dim=0).contiguous()
             self.o_w8 = w8("o_proj").contiguous()
+        # rotary layout of the configuration: part of the head, neighbouring pairs
+        self.rotary_dim = int(self.head_dim * cfg.get("partial_rotary_factor", 1.0))
+        self.rope_interleaved = bool(cfg.get("rope_interleaved", False))
+        self.plain_rope = self.rotary_dim == self.head_dim and not self.rope_interleaved
         self.norm = nn.RMSNorm(self.hidden, eps=cfg["rms_norm_eps"]).to(dev)
         nw = weights.get(pre + "input_layernorm")
         if nw is not None:
@@ -928,7 +934,7 @@ class GroupedQueryAttention(nn.Module):
         # one-token steps as three kernels: RMSNorm + q/k/v GEMV, RoPE + cache write +
         # attention (hc_attn_decode), o GEMV + residual
         self.fused_decode = (self.fp8_decode and self.head_dim == 128 and self.n_q % self.n_kv == 0
-                             and self.n_q // self.n_kv <= 8)
+                             and self.n_q // self.n_kv <= 8 and self.plain_rope)
         self.status = N.new_status(dev)
 
     def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, cache: KVCache,
@@ -941,10 +947,16 @@ class GroupedQueryAttention(nn.Module):
         D, nq, nkv = self.head_dim, self.n_q, self.n_kv
         one = self.fp8_decode and B * T == 1
         qkv = self._gemv(self.qkv_w8, self.norm(x)) if one else F.linear(self.norm(x), self.qkv_weight)
+        if not self.plain_rope:          # rotated in place, among the rows of the projection
+            rows = qkv.view(B * T, nq + 2 * nkv, D)
+            at = torch.arange(T, device=x.device).repeat(B)
+            paged.rope(rows[:, :nq], rows[:, nq:nq + nkv], cos, sin, at, interleaved=self.rope_interleaved,
+                       q_out=rows[:, :nq], k_out=rows[:, nq:nq + nkv])
         q = qkv[..., :nq * D].view(B, T, nq, D).transpose(1, 2)
         k = qkv[..., nq * D:(nq + nkv) * D].view(B, T, nkv, D).transpose(1, 2)
         v = qkv[..., (nq + nkv) * D:].view(B, T, nkv, D).transpose(1, 2)
-        q, k = _rotate(q, cos, sin), _rotate(k, cos, sin)
+        if self.plain_rope:
+            q, k = _rotate(q, cos, sin), _rotate(k, cos, sin)
         kc, vc = cache.k[self.layer_idx], cache.v[self.layer_idx]
         if start is not None:
             kc[:, :, start:start + T] = k
@@ -987,6 +999,24 @@ class GroupedQueryAttention(nn.Module):
         N.check(N.lib.hc_fp8_gemv_ex(N.ptr(self.o_w8), None, self.hidden, self.hidden, N.ptr(att), None, 0.0,
                                      N.ptr(xv), N.ptr(y), s), "hc_fp8_gemv_ex")
         return y
+
+    def step_paged(self, x: torch.Tensor, cos_t: torch.Tensor, sin_t: torch.Tensor, cache: "paged.PagedKVCache",
+                   plan: "paged.PagePlan", max_q: int) -> torch.Tensor:
+        """x + attention(x) for the rows x [rows, H] fp16 of a planned step of many
+        requests: their keys and values go into the paged 8-bit cache and every
+        row attends over its request's pages (hc_rope_append, hc_paged_attn).
+        ``cos_t`` / ``sin_t`` are the whole rotary tables."""
+        n, D, nq, nkv = x.shape[0], self.head_dim, self.n_q, self.n_kv
+        if self.fp8_decode and n == 1:
+            qkv = self._gemv(self.qkv_w8, self.norm(x))
+        else:
+            qkv = F.linear(self.norm(x), self.qkv_weight)
+        rows = qkv.view(n, nq + 2 * nkv, D)
+        q = cache.rope_append(self.layer_idx, rows[:, :nq], rows[:, nq:nq + nkv], rows[:, nq + nkv:], cos_t, sin_t,
+                              plan, interleaved=self.rope_interleaved)
+        out = cache.attend(self.layer_idx, q, plan, max_q=max_q).view(n, nq * D)
+        y = self._gemv(self.o_w8, out).view(n, -1) if self.fp8_decode and n == 1 else F.linear(out, self.o_weight)
+        return x + y
 
     def _attend_one(self, q, keys, vals, mask):
         """Softmax attention of one query position per head, the query heads
@@ -1095,7 +1125,11 @@ class DesdemonaEngine(nn.Module):
             for li in range(self.num_layers)])
         del shared
         self.requires_grad_(False)
-        self.cos_cache, self.sin_cache = build_rope_cache(self.max_seq, self.head_dim, cfg["rope_theta"], dev)
+        rotary, scaling = self.attention_layers[0].rotary_dim, cfg.get("rope_scaling")
+        if scaling or rotary != self.head_dim:
+            self.cos_cache, self.sin_cache = paged.rope_tables(self.max_seq, rotary, cfg["rope_theta"], scaling, dev)
+        else:
+            self.cos_cache, self.sin_cache = build_rope_cache(self.max_seq, self.head_dim, cfg["rope_theta"], dev)
         W = (cfg["intermediate_dim"] + 31) // 32
         self._words = torch.zeros(self.num_layers, 1, W, dtype=torch.int32, device=dev)   # fetch sets in flight
         self.fused_lookahead = True
@@ -1242,6 +1276,89 @@ class DesdemonaEngine(nn.Module):
             for i, t in enumerate(ids):
                 if t in eos:
                     return ids[:i + 1]
+        return ids
+
+    # -- many requests over the paged 8-bit cache ----------------------------
+    def new_paged_cache(self, max_requests: int, n_pages: Optional[int] = None, page_size: int = 64,
+                        max_len: Optional[int] = None) -> "paged.PagedKVCache":
+        """A cache for up to ``max_requests`` requests of up to ``max_len``
+        positions (default: the engine's limit) sharing ``n_pages`` pages
+        (default: enough for all of them at full length)."""
+        length = min(max_len or self.max_seq, self.max_seq)
+        n = n_pages if n_pages is not None else max_requests * -(-length // page_size)
+        return paged.PagedKVCache(self.num_layers, self.cfg["num_key_value_heads"], self.head_dim, n,
+                                  page_size=page_size, max_requests=max_requests, max_len=length, device=self.device)
+
+    @torch.inference_mode()
+    def forward_paged(self, tokens: torch.Tensor, q_lens: Sequence[int], cache: "paged.PagedKVCache") -> torch.Tensor:
+        """Logits [requests with new tokens, vocab] of every request's last row.
+
+        ``q_lens[r]`` new tokens of request r follow its cached ones; ``tokens``
+        [sum(q_lens)] holds them request after request.  All rows share one
+        fetch set per layer, as a batch does in the reference (engine.py:277)."""
+        q_lens = [int(n) for n in q_lens]
+        rows = sum(q_lens)
+        if len(q_lens) > cache.max_requests or tokens.dim() != 1 or tokens.shape[0] != rows or rows == 0 or \
+                min(q_lens) < 0:
+            raise ValueError("tokens must hold sum(q_lens) > 0 ids of at most max_requests requests")
+        device_lens = torch.zeros(cache.max_requests, dtype=torch.int32)
+        device_lens[:len(q_lens)] = torch.tensor(q_lens, dtype=torch.int32)
+        plan = cache.plan(device_lens.to(self.device), rows)
+        x = self.embed_tokens(tokens.to(self.device))
+        f, words, max_q = self.ffn_layers, self._words, max(q_lens)
+        f[0].submit_cold_fetch(x.view(rows, 1, -1), out=words[0])
+        for li, att in enumerate(self.attention_layers):
+            x = att.step_paged(x, self.cos_cache, self.sin_cache, cache, plan, max_q)
+            if li + 1 < self.num_layers:
+                f[li + 1].submit_cold_fetch(x.view(rows, 1, -1), out=words[li + 1])
+            x = f[li](x.view(rows, 1, -1), words[li]).view(rows, -1)
+        cache.commit(plan)
+        last = [e - 1 for e, n in zip(np.cumsum(q_lens).tolist(), q_lens) if n]
+        x = x[torch.tensor(last, device=self.device)]
+        return F.linear(self.final_norm(x), self.lm_head_weight)
+
+    @torch.inference_mode()
+    def generate_batch(self, prompts: Sequence[torch.Tensor], max_new_tokens: int = 200, temperature: float = 0.7,
+                       top_p: float = 0.9, eos_token_id=None, page_size: int = 64) -> list[list[int]]:
+        """generate() for several prompts at once over one paged cache: the
+        generated ids of each, prompt excluded, with generate()'s stopping rule.
+        Finished requests give their pages back and leave the batch (the host
+        looks at the tokens every 16 steps)."""
+        eos = set() if eos_token_id is None else {eos_token_id} if isinstance(eos_token_id, int) else set(eos_token_id)
+        prompts = [p.reshape(-1) for p in prompts]
+        n_new = max(int(max_new_tokens), 1)
+        lens = [p.shape[0] for p in prompts]
+        if not prompts or min(lens) == 0 or max(lens) + n_new > self.max_seq:
+            raise ValueError(f"prompts must be non-empty and fit {self.max_seq} positions with the new tokens")
+        pages = sum(-(-(n + n_new) // page_size) for n in lens)
+        cache = self.new_paged_cache(len(prompts), pages, page_size, max(lens) + n_new)
+        out = torch.empty(len(prompts), n_new, dtype=torch.int64, device=self.device)
+        ids = [[] for _ in prompts]
+        live = list(range(len(prompts)))
+        logits = self.forward_paged(torch.cat([p.to(self.device) for p in prompts]), lens, cache)
+        for step in range(n_new):
+            out[live, step] = _sample(logits, temperature, top_p).view(-1)
+            if step + 1 == n_new:
+                break
+            if eos and step % 16 == 15:
+                made = out[:, :step + 1].tolist()
+                ended = [r for r in live if any(t in eos for t in made[r])]
+                for r in ended:
+                    ids[r] = made[r]
+                if ended:
+                    done = torch.zeros(len(prompts), dtype=torch.bool)
+                    done[ended] = True
+                    cache.release(done.to(self.device))
+                    live = [r for r in live if r not in ended]
+                if not live:
+                    break
+            logits = self.forward_paged(out[live, step], [int(r in live) for r in range(len(prompts))], cache)
+        cache.check()
+        made = out.tolist()
+        for r in range(len(prompts)):
+            row = ids[r] or made[r]
+            stop = next((i for i, t in enumerate(row) if t in eos), len(row) - 1)
+            ids[r] = row[:stop + 1]
         return ids
 
     def check(self):

@@ -23,6 +23,7 @@ is an optional device int32 word that collects HC_ERR_* bits
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import NamedTuple, Optional
 
@@ -35,46 +36,69 @@ PAGE_SIZES = (16, 32, 64, 128)
 
 
 # ─── Argument checks ──────────────────────────────────────────────────────────
+# A step makes three calls a layer, so the checks are plain expressions; what
+# is wrong is put into words only when one of them fails.
+_I32, _I64, _F32, _U8 = torch.int32, torch.int64, torch.float32, torch.uint8
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def _need(ok: bool, what: str):
     if not ok:
         raise ValueError(what)
 
 
-def _tensor(t: torch.Tensor, name: str, dtype, shape, device):
-    """t is a contiguous tensor of this dtype, shape (None: any size) and device."""
-    if t.dtype != dtype or t.dim() != len(shape) or not t.is_contiguous() or t.device != device or \
-            any(n is not None and n != m for n, m in zip(shape, t.shape)):
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {list(shape)} on {device}, got "
-                         f"{t.dtype} {list(t.shape)} on {t.device}"
-                         f"{'' if t.is_contiguous() else ', not contiguous'}")
+def _bad(t: torch.Tensor, name: str, dtype, shape, dev: int):
+    raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on cuda:{dev}, got {t.dtype} "
+                     f"{list(t.shape)} on {t.device}{'' if t.is_contiguous() else ', not contiguous'}")
 
 
-def _heads(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None):
-    """t is [rows, heads, dim] in fp16 or bf16 with contiguous dim (rows and heads may be strided)."""
+def _vector(t: torch.Tensor, name: str, dtype, n: Optional[int], dev: int) -> int:
+    """t is a contiguous vector of n elements (None: any number) on device dev; its address."""
+    if t.dtype is not dtype or t.get_device() != dev or t.dim() != 1 or not t.is_contiguous() or \
+            (n is not None and t.shape[0] != n):
+        _bad(t, name, dtype, [n], dev)
+    return t.data_ptr()
+
+
+def _matrix(t: torch.Tensor, name: str, dtype, n: Optional[int], m: Optional[int], dev: int) -> int:
+    if t.dtype is not dtype or t.get_device() != dev or t.dim() != 2 or not t.is_contiguous() or \
+            (n is not None and t.shape[0] != n) or (m is not None and t.shape[1] != m):
+        _bad(t, name, dtype, [n, m], dev)
+    return t.data_ptr()
+
+
+def _table(t: torch.Tensor, n: int, dev: int) -> int:
+    if t.dtype is not _I32 or t.get_device() != dev or t.dim() != 2 or t.shape[0] != n or t.stride(1) != 1:
+        raise ValueError(f"tables must be int32 [{n}, width] with contiguous rows on cuda:{dev}")
+    return t.data_ptr()
+
+
+def _heads(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None) -> int:
+    """t is [rows, heads, dim] in fp16 or bf16 with contiguous dim (rows and heads may be strided); its address."""
     if not t.is_cuda:
         N.require_cuda(t)
     if t.dim() != 3 or t.dtype not in _DTYPES or (t.stride(2) != 1 and t.shape[2] > 1):
         raise ValueError(f"{name} must be [rows, heads, dim] in float16 or bfloat16 with contiguous dim")
-    if like is not None and (t.dtype != like.dtype or t.device != like.device or t.shape[0] != like.shape[0]
-                             or t.shape[2] != like.shape[2]):
+    if like is not None and (t.dtype is not like.dtype or t.get_device() != like.get_device()
+                             or t.shape[0] != like.shape[0] or t.shape[2] != like.shape[2]):
         raise ValueError(f"{name} must have the rows, dim, dtype and device of the other heads")
+    return t.data_ptr()
 
 
-class _On:
-    """The stream to launch on: the tensor's device made current for the call."""
+def _status(t: Optional[torch.Tensor], dev: int) -> Optional[int]:
+    return None if t is None else _vector(t, "status", _I32, 1, dev)
 
-    def __init__(self, device: torch.device):
-        self.device = device
 
-    def __enter__(self) -> int:
-        self.back = torch.cuda.current_device()
-        if self.device.index != self.back:
-            torch.cuda.set_device(self.device)
-        return torch.cuda.current_stream(self.device).cuda_stream
-
-    def __exit__(self, *exc):
-        if self.device.index != self.back:
-            torch.cuda.set_device(self.back)
+def _call(fn, where: str, dev: int, *args):
+    """fn(*args, stream) with ``dev`` current and its current stream."""
+    back = torch.cuda.current_device()
+    if back == dev:
+        rc = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
+    if rc:
+        raise N.HotColdError(where, rc)
 
 
 # ─── Block tables and slot maps ───────────────────────────────────────────────
@@ -97,24 +121,20 @@ def page_plan(starts: torch.Tensor, q_lens: torch.Tensor, tables: torch.Tensor, 
     of the step's arrays, at least the new tokens; the rest is padding.  When
     the lengths, rows or free pages do not work out, nothing is taken, every
     row is padding and HC_ERR_RANGE is set in ``status``."""
-    N.require_cuda(starts)
-    dev, n = starts.device, starts.shape[0]
-    _tensor(starts, "starts", torch.int32, (None,), dev)
-    _tensor(q_lens, "q_lens", torch.int32, (n,), dev)
-    _tensor(free_pages, "free_pages", torch.int32, (None,), dev)
-    _tensor(n_free, "n_free", torch.int32, (1,), dev)
-    _need(tables.dim() == 2 and tables.shape[0] == n and tables.dtype == torch.int32 and tables.device == dev
-          and tables.stride(1) == 1, "tables must be int32 [requests, width] with contiguous rows")
+    dev, n = starts.get_device(), starts.shape[0]
+    if dev < 0:
+        N.require_cuda(starts)
     _need(n_rows >= 0, "n_rows must not be negative")
-    both = torch.empty(2 * n + 1, dtype=torch.int32, device=dev)
-    rows = torch.empty(2, n_rows, dtype=torch.int64, device=dev)
-    cu_q, kv_lens = both[:n + 1], both[n + 1:]
-    positions, slots = rows[0], rows[1]
-    with _On(dev) as s:
-        N.check(N.lib.hc_page_plan(starts.data_ptr(), q_lens.data_ptr(), n, tables.data_ptr(), tables.stride(0),
-                                   tables.shape[1], free_pages.data_ptr(), free_pages.shape[0], n_free.data_ptr(),
-                                   page_size, n_rows, cu_q.data_ptr(), kv_lens.data_ptr(), positions.data_ptr(),
-                                   slots.data_ptr(), N.ptr(status), s), "hc_page_plan")
+    device = starts.device
+    cu_q = torch.empty(n + 1, dtype=_I32, device=device)
+    kv_lens = torch.empty(n, dtype=_I32, device=device)
+    positions = torch.empty(n_rows, dtype=_I64, device=device)
+    slots = torch.empty(n_rows, dtype=_I64, device=device)
+    _call(N.lib.hc_page_plan, "hc_page_plan", dev, _vector(starts, "starts", _I32, None, dev),
+          _vector(q_lens, "q_lens", _I32, n, dev), n, _table(tables, n, dev), tables.stride(0), tables.shape[1],
+          _vector(free_pages, "free_pages", _I32, None, dev), free_pages.shape[0],
+          _vector(n_free, "n_free", _I32, 1, dev), page_size, n_rows, cu_q.data_ptr(), kv_lens.data_ptr(),
+          positions.data_ptr(), slots.data_ptr(), _status(status, dev))
     return PagePlan(cu_q, kv_lens, positions, slots)
 
 
@@ -122,17 +142,13 @@ def page_release(done: torch.Tensor, tables: torch.Tensor, free_pages: torch.Ten
                  status: Optional[torch.Tensor] = None):
     """Gives the pages of the requests with ``done[r]`` (bool) back to the
     stack and empties their table rows, in place (hc_page_release)."""
-    N.require_cuda(done)
-    dev, n = done.device, done.shape[0]
-    _tensor(done, "done", torch.bool, (None,), dev)
-    _tensor(free_pages, "free_pages", torch.int32, (None,), dev)
-    _tensor(n_free, "n_free", torch.int32, (1,), dev)
-    _need(tables.dim() == 2 and tables.shape[0] == n and tables.dtype == torch.int32 and tables.device == dev
-          and tables.stride(1) == 1, "tables must be int32 [requests, width] with contiguous rows")
-    with _On(dev) as s:
-        N.check(N.lib.hc_page_release(done.data_ptr(), n, tables.data_ptr(), tables.stride(0), tables.shape[1],
-                                      free_pages.data_ptr(), free_pages.shape[0], n_free.data_ptr(), N.ptr(status),
-                                      s), "hc_page_release")
+    dev, n = done.get_device(), done.shape[0]
+    if dev < 0:
+        N.require_cuda(done)
+    _call(N.lib.hc_page_release, "hc_page_release", dev, _vector(done, "done", torch.bool, None, dev), n,
+          _table(tables, n, dev), tables.stride(0), tables.shape[1],
+          _vector(free_pages, "free_pages", _I32, None, dev), free_pages.shape[0],
+          _vector(n_free, "n_free", _I32, 1, dev), _status(status, dev))
 
 
 # ─── Rotary positions ─────────────────────────────────────────────────────────
@@ -191,23 +207,26 @@ def rope_tables(max_seq_len: int, rotary_dim: int, theta: float, scaling: Option
 
 
 def _rope_args(q, k, q_out, k_out, cos, sin, positions, interleaved) -> N.RopeArgs:
-    _heads(q, "q")
-    _heads(k, "k", q)
-    _heads(q_out, "q_out", q)
-    _need(q_out.shape == q.shape, "q_out must have the shape of q")
-    if k_out is not None:
+    qp, kp = _heads(q, "q"), _heads(k, "k", q)
+    rows, nq, dim = q.shape
+    dev = q.get_device()
+    if q_out is not q:
+        _heads(q_out, "q_out", q)
+        _need(q_out.shape[1] == nq, "q_out must have the shape of q")
+    if k_out is not k:
         _heads(k_out, "k_out", q)
-        _need(k_out.shape == k.shape, "k_out must have the shape of k")
-    dev, dim = q.device, q.shape[2]
-    _tensor(cos, "cos", torch.float32, (None, None), dev)
-    _tensor(sin, "sin", torch.float32, cos.shape, dev)
-    _tensor(positions, "positions", torch.int64, (q.shape[0],), dev)
-    _need(0 < 2 * cos.shape[1] <= dim, "cos and sin must cover at most the head")
-    ko = k_out if k_out is not None else k
-    return N.RopeArgs(q.data_ptr(), k.data_ptr(), q_out.data_ptr(), ko.data_ptr(), q.stride(0), q.stride(1),
-                      k.stride(0), k.stride(1), q_out.stride(0), q_out.stride(1), ko.stride(0), ko.stride(1),
-                      cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(), q.shape[0], q.shape[1],
-                      k.shape[1], dim, 2 * cos.shape[1], int(bool(interleaved)), _DTYPES[q.dtype])
+        _need(k_out.shape[1] == k.shape[1], "k_out must have the shape of k")
+    cp = _matrix(cos, "cos", _F32, None, None, dev)
+    length, half = cos.shape
+    sp = _matrix(sin, "sin", _F32, length, half, dev)
+    _need(0 < 2 * half <= dim, "cos and sin must cover at most the head")
+    q0, q1, _ = q.stride()
+    k0, k1, _ = k.stride()
+    r0, r1, _ = q_out.stride()
+    t0, t1, _ = k_out.stride()
+    return N.RopeArgs(qp, kp, q_out.data_ptr(), k_out.data_ptr(), q0, q1, k0, k1, r0, r1, t0, t1, cp, sp, length,
+                      _vector(positions, "positions", _I64, rows, dev), rows, nq, k.shape[1], dim, 2 * half,
+                      1 if interleaved else 0, _DTYPES[q.dtype])
 
 
 def rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor, *,
@@ -220,26 +239,34 @@ def rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
     pass through.  Returns (q_out, k_out), new tensors unless given (q and k
     themselves rotate in place).  Rows at position -1 are left alone."""
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if k_out is None:
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
     args = _rope_args(q, k, q_out, k_out, cos, sin, positions, interleaved)
-    with _On(q.device) as s:
-        N.check(N.lib.hc_rope(ctypes.byref(args), N.ptr(status), s), "hc_rope")
+    dev = q.get_device()
+    _call(N.lib.hc_rope, "hc_rope", dev, ctypes.byref(args), _status(status, dev))
     return q_out, k_out
 
 
 # ─── The cache: write and attention ───────────────────────────────────────────
 def _pages(k_pages, v_pages, k_scale, v_scale) -> N.KVPages:
-    if not k_pages.is_cuda:
+    dev = k_pages.get_device()
+    if dev < 0:
         N.require_cuda(k_pages)
-    dev = k_pages.device
-    _tensor(k_pages, "k_pages", torch.uint8, (None, None, None, None), dev)
-    n, h, p, d = k_pages.shape
-    _tensor(v_pages, "v_pages", torch.uint8, (n, h, p, d), dev)
-    _tensor(k_scale, "k_scale", torch.float32, (n, h), dev)
-    _tensor(v_scale, "v_scale", torch.float32, (n, h), dev)
-    return N.KVPages(k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n, h, p, d)
+    shape = k_pages.shape
+    if k_pages.dtype is not _U8 or len(shape) != 4 or not k_pages.is_contiguous():
+        _bad(k_pages, "k_pages", _U8, "[pages, kv heads, page size, dim]", dev)
+    if v_pages.dtype is not _U8 or v_pages.shape != shape or not v_pages.is_contiguous() or \
+            v_pages.get_device() != dev:
+        _bad(v_pages, "v_pages", _U8, list(shape), dev)
+    n, h, p, d = shape
+    return N.KVPages(k_pages.data_ptr(), v_pages.data_ptr(), _matrix(k_scale, "k_scale", _F32, n, h, dev),
+                     _matrix(v_scale, "v_scale", _F32, n, h, dev), n, h, p, d)
+
+
+def _fits(k: torch.Tensor, v: torch.Tensor, pages: N.KVPages, dev: int):
+    if k.shape != v.shape or k.shape[1] != pages.n_kv_heads or k.shape[2] != pages.head_dim or k.get_device() != dev:
+        raise ValueError("k and v must have the cache's heads, dim and device")
 
 
 def kv_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -250,15 +277,13 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: to
     distinct, the rows of one page follow one another (as page_plan gives
     them); rows with a negative slot are padding."""
     pages = _pages(k_pages, v_pages, k_scale, v_scale)
-    _heads(k, "k")
-    _heads(v, "v", k)
-    _need(k.shape == v.shape and k.shape[1] == pages.n_kv_heads and k.shape[2] == pages.head_dim
-          and k.device == k_pages.device, "k and v must have the cache's heads, dim and device")
-    _tensor(slots, "slots", torch.int64, (k.shape[0],), k.device)
-    with _On(k.device) as s:
-        N.check(N.lib.hc_kv_append(ctypes.byref(pages), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-                                   v.stride(0), v.stride(1), slots.data_ptr(), k.shape[0], _DTYPES[k.dtype],
-                                   N.ptr(status), s), "hc_kv_append")
+    kp, vp, dev = _heads(k, "k"), _heads(v, "v", k), k_pages.get_device()
+    _fits(k, v, pages, dev)
+    k0, k1, _ = k.stride()
+    v0, v1, _ = v.stride()
+    rows = k.shape[0]
+    _call(N.lib.hc_kv_append, "hc_kv_append", dev, ctypes.byref(pages), kp, k0, k1, vp, v0, v1,
+          _vector(slots, "slots", _I64, rows, dev), rows, _DTYPES[k.dtype], _status(status, dev))
 
 
 def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
@@ -268,17 +293,20 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Te
     """:func:`rope` of q and k and :func:`kv_append` of the rotated k and of v
     in one launch (hc_rope_append), with the same results.  Returns q_out."""
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    args = _rope_args(q, k, q_out, None, cos, sin, positions, interleaved)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    args = _rope_args(q, k, q_out, k, cos, sin, positions, interleaved)
     pages = _pages(k_pages, v_pages, k_scale, v_scale)
-    _heads(v, "v", k)
-    _need(k.shape == v.shape and k.shape[1] == pages.n_kv_heads and k.shape[2] == pages.head_dim
-          and k.device == k_pages.device, "k and v must have the cache's heads, dim and device")
-    _tensor(slots, "slots", torch.int64, (k.shape[0],), k.device)
-    with _On(q.device) as s:
-        N.check(N.lib.hc_rope_append(ctypes.byref(args), ctypes.byref(pages), v.data_ptr(), v.stride(0), v.stride(1),
-                                     slots.data_ptr(), N.ptr(status), s), "hc_rope_append")
+    vp, dev = _heads(v, "v", k), k_pages.get_device()
+    _fits(k, v, pages, dev)
+    v0, v1, _ = v.stride()
+    _call(N.lib.hc_rope_append, "hc_rope_append", dev, ctypes.byref(args), ctypes.byref(pages), vp, v0, v1,
+          _vector(slots, "slots", _I64, k.shape[0], dev), _status(status, dev))
     return q_out
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(requests: int, rows: int, heads: int, kv_heads: int, dim: int) -> int:
+    return int(N.lib.hc_paged_attn_workspace_bytes(requests, rows, heads, kv_heads, dim))
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch.Tensor,
@@ -296,32 +324,27 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     of each softmax's sum.  A row that sees no key gives 0 and -inf; padding
     rows of ``out`` are left as they were."""
     pages = _pages(k_pages, v_pages, k_scale, v_scale)
-    _heads(q, "q")
-    dev = q.device
+    qp, dev = _heads(q, "q"), k_pages.get_device()
     rows, heads, dim = q.shape
-    _need(dim == pages.head_dim and dev == k_pages.device and heads % pages.n_kv_heads == 0,
-          "q must have the cache's dim and device, and a multiple of its heads")
+    if dim != pages.head_dim or q.get_device() != dev or heads % pages.n_kv_heads:
+        raise ValueError("q must have the cache's dim and device, and a multiple of its heads")
     n = kv_lens.shape[0]
-    _tensor(kv_lens, "kv_lens", torch.int32, (None,), dev)
-    _tensor(cu_q, "cu_q", torch.int32, (n + 1,), dev)
-    _need(tables.dim() == 2 and tables.shape[0] == n and tables.dtype == torch.int32 and tables.device == dev
-          and tables.stride(1) == 1, "tables must be int32 [requests, width] with contiguous rows")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        op = out.data_ptr()
     else:
-        _heads(out, "out", q)
-        _need(out.shape == q.shape, "out must have the shape of q")
-    if lse is not None:
-        _tensor(lse, "lse", torch.float32, (rows, heads), dev)
-    args = N.AttnArgs(q.data_ptr(), out.data_ptr(), N.ptr(lse), q.stride(0), q.stride(1), out.stride(0),
-                      out.stride(1), tables.data_ptr(), tables.stride(0), tables.shape[1], cu_q.data_ptr(),
-                      kv_lens.data_ptr(), n, rows, int(max_q), heads,
-                      dim ** -0.5 if scale is None else float(scale), _DTYPES[q.dtype])
-    need = N.lib.hc_paged_attn_workspace_bytes(n, rows, heads, pages.n_kv_heads, dim)
-    workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
-    with _On(dev) as s:
-        N.check(N.lib.hc_paged_attn(ctypes.byref(args), ctypes.byref(pages), workspace.data_ptr(),
-                                    workspace.numel(), N.ptr(status), s), "hc_paged_attn")
+        op = _heads(out, "out", q)
+        _need(out.shape[1] == heads, "out must have the shape of q")
+    q0, q1, _ = q.stride()
+    o0, o1, _ = out.stride()
+    args = N.AttnArgs(qp, op, None if lse is None else _matrix(lse, "lse", _F32, rows, heads, dev), q0, q1, o0, o1,
+                      _table(tables, n, dev), tables.stride(0), tables.shape[1],
+                      _vector(cu_q, "cu_q", _I32, n + 1, dev), _vector(kv_lens, "kv_lens", _I32, None, dev), n, rows,
+                      max_q, heads, dim ** -0.5 if scale is None else scale, _DTYPES[q.dtype])
+    need = max(_workspace_bytes(n, rows, heads, pages.n_kv_heads, dim), 16)
+    workspace = torch.empty(need, dtype=_U8, device=q.device)
+    _call(N.lib.hc_paged_attn, "hc_paged_attn", dev, ctypes.byref(args), ctypes.byref(pages), workspace.data_ptr(),
+          need, _status(status, dev))
     return out
 
 
