@@ -570,6 +570,7 @@ int sm_count() {
 constexpr int MAX_GRID = 444;          // workspace sizing: 3 CTAs on each of a B200's 148 SMs
 
 int64_t workspace_need(int head_dim) { return MAX_GRID * 32ll + 2ll * MAX_GRID * 16 * (head_dim + 2) * 4; }
+bool tiled(int64_t rows) { return rows > SMALL; }
 
 template <typename T, int D, int NT>
 int launch(AttnParams& p, void* workspace, cudaStream_t stream) {
@@ -614,7 +615,8 @@ extern "C" int64_t hc_paged_attn_workspace_bytes(int32_t n_requests, int32_t n_r
                                                  int32_t n_kv_heads, int32_t head_dim) {
   if (n_requests <= 0 || n_rows < 0 || n_q_heads <= 0 || n_kv_heads <= 0 || (head_dim != 64 && head_dim != 128))
     return -1;
-  return workspace_need(head_dim);
+  const int64_t rows = (int64_t)n_rows * (n_q_heads / n_kv_heads);
+  return workspace_need(head_dim) + (tiled(rows) ? prefill_workspace(head_dim) : 0);
 }
 
 extern "C" int hc_paged_attn(const hc_attn_args* a, const hc_kv_pages* c, void* workspace, int64_t workspace_bytes,
@@ -636,7 +638,9 @@ extern "C" int hc_paged_attn(const hc_attn_args* a, const hc_kv_pages* c, void* 
     return HC_ERR_UNSUPPORTED;
   if ((int64_t)a->table_width * c->page_size > INT32_MAX) return HC_ERR_ARG;
   if (a->n_rows == 0) return HC_OK;
-  if (!workspace || !aligned(workspace, 16) || workspace_bytes < workspace_need(c->head_dim)) return HC_ERR_ARG;
+  if (!workspace || !aligned(workspace, 16) ||
+      workspace_bytes < hc_paged_attn_workspace_bytes(a->n_requests, a->n_rows, a->n_q_heads, c->n_kv_heads, c->head_dim))
+    return HC_ERR_ARG;
   AttnParams p = {};
   p.q = a->q;
   p.out = a->out;
@@ -665,12 +669,15 @@ extern "C" int hc_paged_attn(const hc_attn_args* a, const hc_kv_pages* c, void* 
   p.status = status;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   // Up to SMALL rows of a request and head the keys are split over the GPU; more fill the tensor cores' tiles.
-  const int64_t rows = (int64_t)a->max_q * p.g;
+  const int64_t rows = (int64_t)min(a->max_q, a->n_rows) * p.g;
   p.rows_from = 0;
   p.rows_to = INT32_MAX;
-  if (rows > SMALL) {
+  if (tiled(rows)) {
+    const int sms = sm_count();
+    if (sms <= 0) return HC_ERR_CUDA;
     p.rows_from = SMALL + 1;
-    const int rc = launch_prefill(p, a->dtype, c->head_dim, s);
+    const int rc = launch_prefill(p, a->dtype, c->head_dim,
+                                  static_cast<uint8_t*>(workspace) + workspace_need(c->head_dim), sms, s);
     if (rc != HC_OK) return rc;
     p.rows_from = 0;
     p.rows_to = SMALL + 1;

@@ -35,6 +35,10 @@ struct AttnParams {
   int rows_from, rows_to;              // requests of rows_from <= q_len * g < rows_to are served
   float* part;                         // [grid][2][RT (D + 2)]: partials of a share's first and last item
   int4* cuts;                          // [grid][2]: the divided item that begins in a share
+  // tiles of 256 rows: pieces of cut tiles
+  int sms;
+  int4* pf_cuts;                       // slots in use; then tile and number of pieces of each slot
+  float* pf_part;                      // [slot][256 (D + 2)]
   int32_t* status;
 };
 
@@ -90,7 +94,8 @@ __device__ __forceinline__ Req request(const AttnParams& p, int r, bool flag) {
   return x;
 }
 
-// rows of 256 (tcgen05) -- hc_paged_prefill.cu
-int launch_prefill(const AttnParams& p, int dtype, int head_dim, cudaStream_t stream);
+// tiles of 256 rows on tcgen05 -- hc_paged_prefill.cu
+int64_t prefill_workspace(int head_dim);
+int launch_prefill(const AttnParams& p, int dtype, int head_dim, void* workspace, int sms, cudaStream_t stream);
 
 }  // namespace hca8

@@ -12,6 +12,11 @@
 // score buffers a group's softmax runs on without waiting for its products,
 // and the tensor cores always have the other group's to do.
 //
+// Few tiles over long contexts would leave SMs idle, so a tile's keys are cut
+// into pieces no longer than an SM's average share of all keys (and than
+// MIN_PIECE); the pieces of a cut tile leave partial softmaxes, which a second
+// kernel joins.
+//
 // Page scales: a key's scale joins the factor of its 16 score columns, a
 // value's scale enters as log2 in the exponent (see hc_paged_attn.cu).
 //
@@ -34,6 +39,7 @@ constexpr int GROUP_ROWS = 128;
 constexpr int ROWS = 2 * GROUP_ROWS;
 constexpr int KT = 128;                // keys per converted tile
 constexpr int HALF = 64;               // keys per score buffer
+constexpr int MIN_PIECE = 16;          // halves of a piece at least: beginning one costs about four
 constexpr int SLICES = KT / 16;        // 16-key slices: no page is smaller
 constexpr uint32_t PF_TRIES = 1u << 22; // a wait gives up after so many tries (each suspends for a while)
 
@@ -234,61 +240,115 @@ template <typename T, int D>
 __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const AttnParams p) {
   using L = Layout<D>;
   extern __shared__ uint8_t raw[];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ Bars bar;
   __shared__ Slice meta[4][SLICES];    // a tile's slot is written again four tiles later: no reader is left by then
   __shared__ uint32_t s_tmem;
-  __shared__ int s_pre[MAX_REQ + 1];
-  __shared__ int s_wsum[PF_THREADS / 32];
+  __shared__ int2 s_pre[MAX_REQ + 1];  // pieces and slots for partials before each request
+  __shared__ int64_t s_wsum[PF_THREADS / 32];
+  __shared__ int s_piece;
   __shared__ Req s_req[KEPT_REQ];
   const int t = threadIdx.x, lane = t & 31, w = __shfl_sync(0xffffffffu, t >> 5, 0);
   const uint32_t smem = (smem_u32(raw) + 1023) & ~1023u;
 
-  // tiles before each request
-  const int per = (p.n_req + PF_THREADS - 1) / PF_THREADS;
-  int sum = 0;
-  for (int i = 0; i < per; ++i) {
-    const int r = t * per + i;
-    if (r >= p.n_req) break;
-    const Req x = request(p, r, blockIdx.x == 0);
-    if (p.n_req <= KEPT_REQ) s_req[r] = x;
-    sum += (x.q_len * p.g + ROWS - 1) / ROWS;
-    s_pre[r + 1] = sum;
-  }
-  int inc = sum;
+  // The step's work in halves sets the piece length; with it, the pieces of each request.
+  auto tiles_of = [&](const Req& x) { return (x.q_len * p.g + ROWS - 1) / ROWS; };
+  auto halves_of = [](int kv) { return (kv + HALF - 1) / HALF; };
+  auto piece_of = [&](int64_t halves) {                 // even
+    const uint64_t share = ((uint64_t)halves + p.sms - 1) / (unsigned)p.sms;
+    return (int)min((uint64_t)(1 << 28), max((uint64_t)MIN_PIECE, share + (share & 1)));
+  };
+  auto units_of = [&](const Req& x, int piece) {        // pieces << 32 | slots
+    const int cuts = max(1, (halves_of(x.kv) + piece - 1) / piece), n = tiles_of(x) * p.nkv * cuts;
+    return ((int64_t)n << 32) + (cuts > 1 ? n : 0);
+  };
+  auto scan = [&](int64_t v) {                          // inclusive, over the warp
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += v;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    return v;
+  };
+  if (p.n_req <= 32) {                                  // a request a lane, one barrier
+    if (w == 0) {
+      Req x = {0, 0, 0};
+      if (lane < p.n_req) s_req[lane] = x = request(p, lane, blockIdx.x == 0);
+      int64_t sum = (int64_t)tiles_of(x) * p.nkv * halves_of(x.kv);
+#pragma unroll
+      for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      const int piece = piece_of(sum);
+      const int64_t upto = scan(lane < p.n_req ? units_of(x, piece) : 0);
+      s_pre[lane + 1] = make_int2((int)(upto >> 32), (int)upto);
+      if (lane == 0) s_pre[0] = make_int2(0, 0), s_piece = piece;
+    }
+    __syncthreads();
+  } else {
+    const int per = (p.n_req + PF_THREADS - 1) / PF_THREADS;
+    auto mine = [&](int i) {
+      const int r = t * per + i;
+      return p.n_req <= KEPT_REQ ? s_req[r] : request(p, r, false);
+    };
+    const int count = max(0, min(per, p.n_req - t * per));
+    int64_t sum = 0;
+    for (int i = 0; i < count; ++i) {
+      const Req x = request(p, t * per + i, blockIdx.x == 0);
+      if (p.n_req <= KEPT_REQ) s_req[t * per + i] = x;
+      sum += (int64_t)tiles_of(x) * p.nkv * halves_of(x.kv);
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) s_wsum[w] = sum;
+    __syncthreads();
+    sum = 0;
+    for (int k = 0; k < PF_THREADS / 32; ++k) sum += s_wsum[k];
+    __syncthreads();
+    const int piece = piece_of(sum);
+    int64_t own = 0;
+    for (int i = 0; i < count; ++i) own += units_of(mine(i), piece);
+    const int64_t upto = scan(own);
+    if (lane == 31) s_wsum[w] = upto;
+    if (t == 0) s_pre[0] = make_int2(0, 0), s_piece = piece;
+    __syncthreads();
+    int64_t at = upto - own;
+    for (int k = 0; k < w; ++k) at += s_wsum[k];
+    for (int i = 0; i < count; ++i) {
+      at += units_of(mine(i), piece);
+      s_pre[t * per + i + 1] = make_int2((int)(at >> 32), (int)at);
+    }
+    __syncthreads();
   }
-  if (lane == 31) s_wsum[w] = inc;
-  if (t == 0) s_pre[0] = 0;
-  __syncthreads();
-  int base = inc - sum, total = 0;
-  for (int k = 0; k < PF_THREADS / 32; ++k) {
-    if (k < w) base += s_wsum[k];
-    total += s_wsum[k];
-  }
-  for (int i = 0; i < per; ++i) {
-    const int r = t * per + i;
-    if (r >= p.n_req) break;
-    s_pre[r + 1] += base;
-  }
-  __syncthreads();
+  const int piece = s_piece, all = s_pre[p.n_req].x;
+  if (blockIdx.x == 0 && t == 0) p.pf_cuts[0] = make_int4(s_pre[p.n_req].y, 0, 0, 0);
   // later tiles see more keys: they start first
-  const int h = blockIdx.x % p.nkv, tile = total - 1 - blockIdx.x / p.nkv;
-  if (tile < 0) return;
+  const int unit = all - 1 - (int)blockIdx.x;
+  if (unit < 0) return;
   int r = 0;
   for (int b = p.n_req; b - r > 1;) {
     const int mid = (r + b) / 2;
-    if (s_pre[mid] <= tile) r = mid;
+    if (s_pre[mid].x <= unit) r = mid;
     else b = mid;
   }
   const Req x = p.n_req <= KEPT_REQ ? s_req[r] : request(p, r, false);
-  const int row0 = (tile - s_pre[r]) * ROWS;
+  const unsigned cuts = max(1, (halves_of(x.kv) + piece - 1) / piece);
+  const unsigned in = unit - s_pre[r].x;               // (tile, key-value head, piece)
+  const int cut = in % cuts, h = in / cuts % p.nkv, row0 = (int)(in / cuts / p.nkv) * ROWS;
+  const int slot = s_pre[r].y + (int)in;
   const int n_here = min(ROWS, x.q_len * p.g - row0);
-  const int behind = x.kv - x.q_len;
-  const int lim_hi = behind + (row0 + n_here - 1) / p.g;         // last key that any row sees
-  const int n_tiles = lim_hi < 0 ? 0 : lim_hi / KT + 1, n_half = lim_hi < 0 ? 0 : lim_hi / HALF + 1;
+  const int lim_last = x.kv - x.q_len + (row0 + n_here - 1) / p.g;       // last key that any row sees
+  const int tile_half = lim_last < 0 ? 0 : lim_last / HALF + 1;          // halves of the tile
+  const int n_cut = max(1, (tile_half + piece - 1) / piece);             // pieces that have any
+  const bool split = n_cut > 1;
+  if (cuts > 1 && t == 0) {
+    p.pf_cuts[1 + 2 * slot] = make_int4(row0, n_here, x.q0, h);
+    p.pf_cuts[2 + 2 * slot] = make_int4(split && cut == 0 ? n_cut : 0, 0, 0, 0);
+  }
+  if (cut >= n_cut) return;
+  // from here on keys count from the piece's first
+  const int key_first = cut * piece * HALF;
+  const int n_half = min(tile_half - cut * piece, piece), n_tiles = (n_half + 1) / 2;
+  const int behind = x.kv - x.q_len - key_first, lim_hi = min(lim_last - key_first, n_half * HALF - 1);
+  const int32_t* table = p.tables + (int64_t)r * p.t_stride + (key_first >> p.page_log2);
   const bool two = n_here > GROUP_ROWS;
 
   if (w == MMA_WARP) {
@@ -457,6 +517,20 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
         ok = __all_sync(0xffffffffu, ok);
         fence_after();
       }
+      if (split) {                                      // a partial: [D / 4][256 rows] of four dims, then m and l
+        float* part = p.pf_part + (int64_t)slot * (ROWS * (D + 2));
+#pragma unroll 1
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          if (!ok) break;
+          tmem_ld32(at_o + c0, s);
+          tmem_wait_ld(s);
+#pragma unroll
+          for (int c = 0; c < 32; c += 4)
+            reinterpret_cast<uint4*>(part)[(c0 + c) / 4 * ROWS + t] = make_uint4(s[c], s[c + 1], s[c + 2], s[c + 3]);
+        }
+        part[ROWS * D + t] = m;
+        part[ROWS * D + ROWS + t] = l;
+      } else {
       // The warp's 32 rows go through its part of the query tile (no product reads it any more), so that a
       // store instruction writes whole rows.
       const float inv = l > 0.0f ? __frcp_rn(l) : l;    // no key: 0, and NaN stays NaN
@@ -506,6 +580,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
         }
       }
       if (out_at >= 0 && p.lse) p.lse[lse_at] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * LN2;
+      }
     }
   } else if (w < MMA_WARP) {
     // ---- converters: e4m3 pages -> f16 operand tiles -------------------------
@@ -516,7 +591,6 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
     uint4 kr[N], vr[N];
     // Page of the slice that holds a key.  Keys behind lim_hi read the page of
     // lim_hi: their bytes are replaced before they are converted.
-    const int32_t* table = p.tables + (int64_t)r * p.t_stride;
     auto page_of = [&](int key) { return __ldg(table + (min(key, lim_hi) >> p.page_log2)); };
     // A thread's pieces lie in N slices; it reads their pages itself, a tile
     // ahead: shuffles between the loads made each wait for the one before.
@@ -607,7 +681,6 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
     }
   } else if (w == SCALE_WARP) {
     // ---- scales: lane l has slice l of a tile; pages and scales run ahead ------
-    const int32_t* table = p.tables + (int64_t)r * p.t_stride;
     const int key = (lane & (SLICES - 1)) * 16;
     auto page_of = [&](int j) { return __ldg(table + (min(j * KT + key, lim_hi) >> p.page_log2)); };
     auto head_of = [&](int page) { return (int64_t)((unsigned)page < (unsigned)p.n_pages ? page : 0) * p.nkv + h; };
@@ -713,23 +786,96 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
+// Joins the pieces of the tiles that were cut: a thread has a row and 16 dims.
 template <typename T, int D>
-int launch_pf(const AttnParams& p, cudaStream_t stream) {
+__global__ void __launch_bounds__(ROWS) paged_prefill_join_kernel(const AttnParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int t = threadIdx.x, slots = p.pf_cuts[0].x;
+  for (int slot = blockIdx.x; slot < slots; slot += gridDim.x) {
+    const int n = p.pf_cuts[2 + 2 * slot].x;
+    const int4 tile = p.pf_cuts[1 + 2 * slot];           // first row, rows, first token, key-value head
+    if (n == 0 || t >= tile.y) continue;
+    const int64_t stride = ROWS * (D + 2);
+    const float* part = p.pf_part + slot * stride;
+    float M = M_NONE, L = 0.0f;
+    for (int k = 0; k < n; ++k) M = fmaxf(M, part[k * stride + ROWS * D + t]);
+    float a[16];
+#pragma unroll
+    for (int c = 0; c < 16; ++c) a[c] = 0.0f;
+#pragma unroll 2
+    for (int k = 0; k < n; ++k) {
+      const float* q = part + k * stride;
+      const float f = ex2(q[ROWS * D + t] - M);
+      L = fmaf(q[ROWS * D + ROWS + t], f, L);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float4 v = reinterpret_cast<const float4*>(q)[(4 * blockIdx.y + c) * ROWS + t];
+        // a piece that the row sees nothing of adds nothing, whatever its sums hold
+        a[4 * c] = fmaf(v.x, f, a[4 * c]);
+        a[4 * c + 1] = fmaf(v.y, f, a[4 * c + 1]);
+        a[4 * c + 2] = fmaf(v.z, f, a[4 * c + 2]);
+        a[4 * c + 3] = fmaf(v.w, f, a[4 * c + 3]);
+      }
+    }
+    const float inv = L > 0.0f ? __frcp_rn(L) : L;
+    const int tok = tile.z + (tile.x + t) / p.g, head = tile.w * p.g + (tile.x + t) % p.g;
+    T* out = static_cast<T*>(p.out) + (int64_t)tok * p.o_row + head * p.o_head + 16 * blockIdx.y;
+    uint32_t o[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) o[c] = L == 0.0f ? 0u : pack2<T>(a[2 * c] * inv, a[2 * c + 1] * inv);
+    if ((reinterpret_cast<uintptr_t>(out) & 15) == 0) {
+      reinterpret_cast<uint4*>(out)[0] = make_uint4(o[0], o[1], o[2], o[3]);
+      reinterpret_cast<uint4*>(out)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+    } else {
+      const T* e = reinterpret_cast<const T*>(o);
+#pragma unroll
+      for (int c = 0; c < 16; ++c) out[c] = e[c];
+    }
+    if (p.lse && blockIdx.y == 0)
+      p.lse[(int64_t)tok * p.nq + head] = L == 0.0f ? -INFINITY : (M + __log2f(L)) * LN2;
+  }
+}
+
+// Slots for partials: a request that is cut has under twice its work over the piece length, and a piece is at
+// least an SM's share of all work.
+constexpr int MAX_SMS = 148, MAX_SLOTS = 2 * MAX_SMS;
+
+int64_t prefill_workspace(int head_dim) { return 16 * (1 + 2 * MAX_SLOTS) + (int64_t)MAX_SLOTS * ROWS * (head_dim + 2) * 4; }
+
+template <typename T, int D>
+int launch_pf(AttnParams p, void* workspace, int sms, cudaStream_t stream) {
   using L = Layout<D>;
+  p.sms = min(sms, MAX_SMS);
+  p.pf_cuts = static_cast<int4*>(workspace);
+  p.pf_part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + 16 * (1 + 2 * MAX_SLOTS));
   if (cudaFuncSetAttribute(paged_prefill_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::BYTES) !=
       cudaSuccess)
     return HC_ERR_CUDA;
-  // the lengths are on the device: as many tiles as any lengths of these rows can need
+  // the lengths are on the device: as many pieces as any lengths of these rows can need
   const int64_t tiles = ((int64_t)p.n_rows * p.g + ROWS - 1) / ROWS + min(p.n_req, p.n_rows);
-  if (tiles * p.nkv > INT32_MAX) return HC_ERR_UNSUPPORTED;
-  paged_prefill_kernel<T, D><<<(unsigned)(tiles * p.nkv), PF_THREADS, L::BYTES, stream>>>(p);
-  return cudaGetLastError() == cudaSuccess ? HC_OK : HC_ERR_CUDA;
+  const int64_t pieces = tiles * p.nkv + p.sms;
+  if (pieces > INT32_MAX) return HC_ERR_UNSUPPORTED;
+  paged_prefill_kernel<T, D><<<(unsigned)pieces, PF_THREADS, L::BYTES, stream>>>(p);
+  if (cudaGetLastError() != cudaSuccess) return HC_ERR_CUDA;
+  if (((int64_t)p.width << p.page_log2) <= MIN_PIECE * HALF) return HC_OK;       // no length that the tables hold is cut
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(MAX_SMS / 2, D / 16);
+  cfg.blockDim = dim3(ROWS);
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_prefill_join_kernel<T, D>, p) == cudaSuccess ? HC_OK : HC_ERR_CUDA;
 }
 
-int launch_prefill(const AttnParams& p, int dtype, int head_dim, cudaStream_t stream) {
+int launch_prefill(const AttnParams& p, int dtype, int head_dim, void* workspace, int sms, cudaStream_t stream) {
   if (dtype == HC_F16)
-    return head_dim == 128 ? launch_pf<__half, 128>(p, stream) : launch_pf<__half, 64>(p, stream);
-  return head_dim == 128 ? launch_pf<__nv_bfloat16, 128>(p, stream) : launch_pf<__nv_bfloat16, 64>(p, stream);
+    return head_dim == 128 ? launch_pf<__half, 128>(p, workspace, sms, stream)
+                           : launch_pf<__half, 64>(p, workspace, sms, stream);
+  return head_dim == 128 ? launch_pf<__nv_bfloat16, 128>(p, workspace, sms, stream)
+                         : launch_pf<__nv_bfloat16, 64>(p, workspace, sms, stream);
 }
 
 }  // namespace hca8

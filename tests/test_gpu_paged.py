@@ -483,6 +483,29 @@ def test_paged_attention_long_contexts_are_split(P, N, nq, nkv, dim, spans):
     _check_attention(out, lse, q, cache, tables, cu, kv)
 
 
+@pytest.mark.parametrize("nq,nkv,dim,page,dtype,spans", [
+    (8, 2, 128, 64, torch.float16, [(9000, 40)]), (8, 1, 64, 128, torch.bfloat16, [(5000, 64), (3, 20), (4097, 9)]),
+    (4, 1, 128, 16, torch.bfloat16, [(2600, 300), (1500, 1), (1, 1)]), (4, 2, 64, 32, torch.float16, [(1030, 1030)]),
+])
+def test_paged_attention_rows_over_long_contexts_are_cut(P, N, nq, nkv, dim, page, dtype, spans):
+    """Few tiles of many rows over long contexts: their keys are cut into pieces that are joined;
+    rows near the diagonal see part of the last piece only."""
+    g = _gen(dim + nq + page)
+    tables, cu, kv, n_pages = _step(spans, page, g)
+    cache = _filled(n_pages, nkv, page, dim, g, spread=1)
+    rows = int(cu[-1])
+    q = torch.randn(rows + 2, nq, dim, generator=g, device="cuda").to(dtype)
+    out, lse = torch.full_like(q, 9.0), torch.full(q.shape[:2], 9.0, device="cuda")
+    st = N.new_status("cuda")
+    P.paged_attention(q, *cache, tables, cu, kv, max_q=max(n for _, n in spans), out=out, lse=lse, status=st)
+    N.read_status(st, "paged_attention")
+    assert (out[rows:] == 9).all() and (lse[rows:] == 9).all()
+    _check_attention(out, lse, q, cache, tables, cu, kv)
+    wide = torch.zeros(rows + 2, nq, dim + 1, device="cuda").to(dtype)[:, :, 1:]              # outputs at odd addresses
+    P.paged_attention(q, *cache, tables, cu, kv, max_q=max(n for _, n in spans), out=wide)
+    assert torch.equal(wide[:rows], out[:rows])
+
+
 def test_paged_attention_strides_scale_and_large_queries(P, N):
     page, nq, nkv, dim = 32, 8, 4, 64
     g = _gen(11)
