@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const RopeArgs p) {
 // the write of a step's keys and values
 // ---------------------------------------------------------------------------
 constexpr int E_MIN = -40, E_MAX = 40;  // exponents of a page scale
-constexpr int CHUNK = 16;               // rows a warp holds at once
+constexpr int MANY = 16, FEW = 4;       // rows a warp holds at once
 constexpr int SPLIT_ROWS = 1024;        // rows from which the queries get a launch of their own
 constexpr int APPEND_THREADS = 256;
 constexpr int APPEND_WARPS = APPEND_THREADS / 32;
@@ -504,15 +504,24 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   return r;
 }
 
+// What a warp read of the rows from t0 on: lane l has row t0 + l.
+struct Window {
+  int t0;
+  int64_t slot, pos;
+};
+
 // Writes one run (the consecutive rows that enter one page) of one head's keys
-// or values: `wpi` warps, each with 16 rows in registers (EL elements of a row
-// per lane), so a run of up to 16 wpi rows is read once and a longer one twice;
+// or values: `wpi` warps, each with ROWS rows in registers (EL elements of a row
+// per lane), so a run of up to ROWS wpi rows is read once and a longer one twice;
 // the warps' largest values meet in shared memory.  The angles of a warp's rows
-// come through shared memory, all copies in flight at once.  Latency-bound.
+// come through shared memory, all copies in flight at once.  What bounds it is
+// latency: the chain slot -> position -> angles and row -> scale.  With 16 rows a
+// warp prompts have the most loads in flight (2 CTAs on an SM); 4 rows need half
+// the registers, and a decode step's single rows have twice the CTAs.
 // Every warp of the block calls it for the same run (`idle`: without an item).
-template <typename T, int EL, bool VEC, bool ROPE>
+template <typename T, int EL, int ROWS, bool VEC, bool ROPE>
 __device__ __forceinline__ void append_run(const AppendArgs& p, int which, int head, int wi, bool idle, float* s_top,
-                                           float* angles, int row0, int n, int64_t slot0) {
+                                           float* angles, const Window& win, int row0, int n, int64_t slot0) {
   constexpr int D = 32 * EL;
   const int lane = threadIdx.x & 31;
   const int64_t page = slot0 >> p.page_log2;
@@ -522,7 +531,7 @@ __device__ __forceinline__ void append_run(const AppendArgs& p, int which, int h
   const T* src = static_cast<const T*>(p.src[which]) + head * p.src_head[which];
   const int64_t step = p.src_row[which];
   const float old = lo && !idle ? *scale_at : 0.0f;  // a run from the page's first row begins the page anew
-  const int d0 = EL * lane, span = CHUNK * p.wpi;
+  const int d0 = EL * lane, span = ROWS * p.wpi;
   if (idle) n = 0;
 
   auto load = [&](int row, T (&x)[EL]) {
@@ -561,7 +570,8 @@ __device__ __forceinline__ void append_run(const AppendArgs& p, int which, int h
 #pragma unroll
       for (int e = 0; e < EL; ++e) o[e] = x[e];
 #pragma unroll
-      for (int e = 0; e < EL; ++e) x[e] = turn_key<T>(o[e], o[e ^ 1], c[e / 2], e & 1 ? c[half + e / 2] : -c[half + e / 2]);
+      for (int e = 0; e < EL; ++e)
+        x[e] = turn_key<T>(o[e], o[e ^ 1], c[e / 2], e & 1 ? c[half + e / 2] : -c[half + e / 2]);
     }
   };
   // the same for any rotary size and alignment
@@ -579,19 +589,21 @@ __device__ __forceinline__ void append_run(const AppendArgs& p, int which, int h
     }
   };
   // rows j0 .. of the run, all loads in flight before the first is used
-  T x[CHUNK][EL];
+  T x[ROWS][EL];
   auto load_chunk = [&](int j0) {
     const int m = n - j0, row = row0 + j0;
     int64_t pos = 0;
     if constexpr (ROPE) {
       if (which == 0) {
-        pos = p.positions[row + min(lane & (CHUNK - 1), m - 1)];
+        const int at = row + min(lane & (ROWS - 1), m - 1), ahead = row - win.t0;
+        if (ahead <= 32 - ROWS) pos = __shfl_sync(0xffffffffu, win.pos, (at - win.t0) & 31);
+        else pos = p.positions[at];
         if constexpr (VEC) {                           // lane l copies piece l of a row's cosines and sines
           const bool sine = 4 * lane >= half;
           const float* table = sine ? p.sin_t + 4 * lane - half : p.cos_t + 4 * lane;
           const uint32_t to = smem_u32(angles) + 16 * lane;
 #pragma unroll
-          for (int j = 0; j < CHUNK; ++j) {
+          for (int j = 0; j < ROWS; ++j) {
             const int64_t at = __shfl_sync(0xffffffffu, pos, j);
             if (j < m && 2 * lane < half)
               asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(to + j * D * 4), "l"(table + at * half)
@@ -601,7 +613,7 @@ __device__ __forceinline__ void append_run(const AppendArgs& p, int which, int h
       }
     }
 #pragma unroll
-    for (int j = 0; j < CHUNK; ++j)
+    for (int j = 0; j < ROWS; ++j)
       if (j < m) load(row + j, x[j]);
     if constexpr (ROPE) {
       if (which == 0) {
@@ -609,12 +621,12 @@ __device__ __forceinline__ void append_run(const AppendArgs& p, int which, int h
           asm volatile("cp.async.wait_all;" ::: "memory");
           __syncwarp();
 #pragma unroll
-          for (int j = 0; j < CHUNK; ++j)
+          for (int j = 0; j < ROWS; ++j)
             if (j < m) rotate(angles + j * D, x[j]);
           __syncwarp();
         } else {
 #pragma unroll
-          for (int j = 0; j < CHUNK; ++j)
+          for (int j = 0; j < ROWS; ++j)
             if (j < m) rotate_any(row + j, __shfl_sync(0xffffffffu, pos, j), x[j]);
         }
       }
@@ -623,10 +635,10 @@ __device__ __forceinline__ void append_run(const AppendArgs& p, int which, int h
   // largest finite value of the run
   float top = 0.0f;
   bool odd = false;
-  for (int j0 = CHUNK * wi; j0 < n; j0 += span) {
+  for (int j0 = ROWS * wi; j0 < n; j0 += span) {
     load_chunk(j0);
 #pragma unroll
-    for (int j = 0; j < CHUNK; ++j)
+    for (int j = 0; j < ROWS; ++j)
       if (j0 + j < n) {
 #pragma unroll
         for (int e = 0; e < EL; ++e) {
@@ -667,10 +679,10 @@ __device__ __forceinline__ void append_run(const AppendArgs& p, int which, int h
     }
   }
   if (wi == 0 && lane == 0 && (grown || !lo)) *scale_at = now;
-  for (int j0 = CHUNK * wi; j0 < n; j0 += span) {
+  for (int j0 = ROWS * wi; j0 < n; j0 += span) {
     if (n > span) load_chunk(j0);
 #pragma unroll
-    for (int j = 0; j < CHUNK; ++j)
+    for (int j = 0; j < ROWS; ++j)
       if (j0 + j < n) {
         float f[EL];
 #pragma unroll
@@ -704,54 +716,56 @@ __device__ __forceinline__ int64_t checked_slot(const AppendArgs& p, int t, bool
 // Runs that begin among rows [t0, t1), t1 - t0 <= 32: a row begins one unless
 // the row before it lies in the same page.  Rows of a page that do not follow
 // one another are flagged and left out.  The whole block works on one run.
-template <typename T, int EL, bool VEC, bool ROPE>
+template <typename T, int EL, int ROWS, bool VEC, bool ROPE>
 __device__ __forceinline__ void append_rows(const AppendArgs& p, int t0, int t1, int item, int wi,
                                             float (*s_top)[APPEND_WARPS], float* angles) {
   const int lane = threadIdx.x & 31, which = item & 1;
   const bool idle = item >= 2 * p.n_kv, flag = item == 0 && wi == 0;
   const int head = idle ? 0 : item >> 1;
+  // 32 rows' slots and positions at once: most runs need no second look
+  Window win = {t0, -1, 0};
   const int mine = t0 + lane;
-  int64_t slot = -1;
-  bool begins = false;
-  if (mine < t1) {
-    slot = checked_slot<ROPE>(p, mine, flag);
-    const int64_t before = mine ? checked_slot<ROPE>(p, mine - 1, false) : -1;
-    const bool same = slot >= 0 && before >= 0 && before >> p.page_log2 == slot >> p.page_log2;
-    begins = slot >= 0 && !same;
-    if (same && before + 1 != slot && flag && p.status) atomicOr(p.status, HC_ERR_RANGE);
+  if (mine < p.n_rows) {
+    win.slot = checked_slot<ROPE>(p, mine, flag && mine < t1);
+    if constexpr (ROPE) win.pos = p.positions[mine];
   }
+  int64_t before = __shfl_up_sync(0xffffffffu, win.slot, 1);
+  if (lane == 0) before = t0 ? checked_slot<ROPE>(p, t0 - 1, false) : -1;
+  const bool same = win.slot >= 0 && before >= 0 && before >> p.page_log2 == win.slot >> p.page_log2;
+  const bool begins = win.slot >= 0 && !same && mine < t1;
+  if (same && before + 1 != win.slot && mine < t1 && flag && p.status) atomicOr(p.status, HC_ERR_RANGE);
   int turn = 0;
   for (uint32_t todo = __ballot_sync(0xffffffffu, begins); todo; todo &= todo - 1) {
     const int from = __ffs(todo) - 1, t = t0 + from;
-    const int64_t first = __shfl_sync(0xffffffffu, slot, from);
+    const int64_t first = __shfl_sync(0xffffffffu, win.slot, from);
     const int left = min(p.page_size - ((int)first & (p.page_size - 1)), p.n_rows - t);
-    int n = 0;
-    for (int base = 0; base < left; base += 32) {
+    const uint32_t follow = __ballot_sync(0xffffffffu, lane >= from && win.slot == first + (lane - from)) >> from;
+    int n = min(left, follow == 0xffffffffu ? 32 : __ffs(~follow) - 1);
+    for (int base = n; n == base && base < left && base >= 32 - from; base += 32) {
       const int j = base + lane;
       const bool follows = j < left && checked_slot<ROPE>(p, t + j, false) == first + j;
       const uint32_t ok = __ballot_sync(0xffffffffu, follows);
       n += ok == 0xffffffffu ? 32 : __ffs(~ok) - 1;
-      if (ok != 0xffffffffu) break;
     }
-    append_run<T, EL, VEC, ROPE>(p, which, head, wi, idle, s_top[turn ^= 1], angles, t, n, first);
+    append_run<T, EL, ROWS, VEC, ROPE>(p, which, head, wi, idle, s_top[turn ^= 1], angles, win, t, n, first);
   }
 }
 
 // n_append blocks write the cache, the others rotate the queries; the two kinds
 // alternate over the grid, since one is bound by latency and the other by HBM.
-template <typename T, int EL, bool VEC, bool ROPE>
-__global__ void __launch_bounds__(APPEND_THREADS, 2) append_kernel(const AppendArgs p, const RopeArgs rope,
-                                                                unsigned n_append, unsigned groups) {
+template <typename T, int EL, int ROWS, bool VEC, bool ROPE>
+__global__ void __launch_bounds__(APPEND_THREADS, ROWS == FEW ? 4 : 2)
+    append_kernel(const AppendArgs p, const RopeArgs rope, unsigned n_append, unsigned groups) {
   const unsigned before = (unsigned)((uint64_t)blockIdx.x * n_append / gridDim.x);
   const unsigned upto = (unsigned)((uint64_t)(blockIdx.x + 1) * n_append / gridDim.x);
   if (upto > before) {
-    extern __shared__ __align__(16) float s_angles[];                // [warp][CHUNK][dim]
+    extern __shared__ __align__(16) float s_angles[];                // [warp][ROWS][dim]
     __shared__ float s_top[2][APPEND_WARPS];
     const int w = threadIdx.x >> 5;
     const int item = (int)(before % groups) * (APPEND_WARPS / p.wpi) + w / p.wpi;
     const int t0 = (int)(before / groups) * p.seg;
-    append_rows<T, EL, VEC, ROPE>(p, t0, min(p.n_rows, t0 + p.seg), item, w % p.wpi, s_top,
-                                  s_angles + w * CHUNK * 32 * EL);
+    append_rows<T, EL, ROWS, VEC, ROPE>(p, t0, min(p.n_rows, t0 + p.seg), item, w % p.wpi, s_top,
+                                  s_angles + w * ROWS * 32 * EL);
     if (p.beside) asm volatile("griddepcontrol.wait;" ::: "memory");   // the queries' kernel ends no later than this
     return;
   }
@@ -783,7 +797,8 @@ int check_rope(const hc_rope_args* a, bool to_cache) {
 
 // The vector form wants 16-byte pieces throughout and whole units of 8 pairs.
 bool rope_vec(const hc_rope_args* a, bool keys) {
-  bool ok = multiple(a->rotary_dim, 16) && multiple(a->head_dim, 16) && a->head_dim <= 16 * ROPE_THREADS && aligned(a->q, 16) && aligned(a->q_out, 16) &&
+  bool ok = multiple(a->rotary_dim, 16) && multiple(a->head_dim, 16) && a->head_dim <= 16 * ROPE_THREADS &&
+            aligned(a->q, 16) && aligned(a->q_out, 16) &&
             multiple(a->q_row, 8) && multiple(a->q_head, 8) && multiple(a->q_out_row, 8) &&
             multiple(a->q_out_head, 8) && aligned(a->cos_t, 16) && aligned(a->sin_t, 16);
   if (keys)
@@ -845,7 +860,7 @@ int check_pages(const hc_kv_pages* c) {
   return HC_OK;
 }
 
-template <typename T>
+template <typename T, int ROWS>
 int launch_append(AppendArgs& p, const hc_rope_args* rope, const hc_kv_pages* c, cudaStream_t stream) {
   RopeArgs ra = {};
   int64_t extra = 0;
@@ -857,17 +872,26 @@ int launch_append(AppendArgs& p, const hc_rope_args* rope, const hc_kv_pages* c,
     ra = rope_args(rope, false, p.status);
     extra = rope_blocks(ra, vec);
   }
-  // Rows a CTA searches: one while rows are few (decode: every row is a run), about a page for prompts.
-  p.seg = max(1, min(min(32, c->page_size), p.n_rows / 256));
-  // Warps of an item: enough to hold a whole page when rows are many; with few, most runs are single rows and
-  // more warps only wait.
-  p.wpi = min(c->page_size / CHUNK, p.n_rows <= 256 ? 1 : p.n_rows < SPLIT_ROWS ? 2 : 8);
+  // Rows a CTA searches.  Few rows: one each, since in a decode step every row is a run (1,000 single rows take
+  // 35 us so, 152 us with 16 rows a warp).  Many: up to a page, for which the CTAs do not outnumber the runs so much
+  // (prompts of 12,288 rows: 57 us; 73 us when every eighth row has its CTAs).
+  p.seg = ROWS == FEW ? 1 : max(1, min(min(32, c->page_size), p.n_rows / 256));
+  // Warps of an item.  Many rows: enough to hold a whole page.  Few: a run may be one row or a page, and the host
+  // does not know which; more warps shorten long runs and make single rows wait.  8 heads, with 1, 2, 4, 8 warps:
+  // 64 single rows 5.3, 5.9, 6.3, 9.4 us, one run of 64 rows 33, 19, 11, 8; 500 single rows 14, 20, 31, 51, one
+  // run of 400 44, 29, 22, 26.  So 8 while all of them fit twice over on the GPU, at least 2.
+  p.wpi = c->page_size / ROWS;
+  if constexpr (ROWS == FEW) {
+    p.wpi = min(p.wpi, APPEND_WARPS);
+    while (p.wpi > 2 && (int64_t)p.n_rows * 2 * p.n_kv * p.wpi > 148 * 16) p.wpi /= 2;
+  }
   const int items = APPEND_WARPS / p.wpi;
   const int groups = (2 * p.n_kv + items - 1) / items;
   const int64_t n_append = (int64_t)((p.n_rows + p.seg - 1) / p.seg) * groups;
   // Few rows: one launch does both.  Many: the queries' rotation needs half of the registers that the write
-  // does, and runs faster as a kernel of its own, which the write may run beside.
-  if (rope && p.n_rows >= SPLIT_ROWS) {
+  // does, and runs faster as a kernel of its own, which the write may run beside (12,288 rows of prompts with 32
+  // query heads: 57 us, 84 in one launch).
+  if (rope && ROWS == MANY) {
     if (vec) rope_kernel<T, true><<<(unsigned)extra, ROPE_THREADS, 0, stream>>>(ra);
     else rope_kernel<T, false><<<(unsigned)extra, ROPE_THREADS, 0, stream>>>(ra);
     if (cudaGetLastError() != cudaSuccess) return HC_ERR_CUDA;
@@ -878,7 +902,7 @@ int launch_append(AppendArgs& p, const hc_rope_args* rope, const hc_kv_pages* c,
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(n_append + extra));
   cfg.blockDim = dim3(APPEND_THREADS);
-  cfg.dynamicSmemBytes = rope && vec ? APPEND_WARPS * CHUNK * c->head_dim * 4 : 0;
+  cfg.dynamicSmemBytes = rope && vec ? APPEND_WARPS * ROWS * c->head_dim * 4 : 0;
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -887,10 +911,11 @@ int launch_append(AppendArgs& p, const hc_rope_args* rope, const hc_kv_pages* c,
   cfg.numAttrs = p.beside ? 1 : 0;
   cudaError_t rc;
 #define GO(EL, V, R)                                                                                          \
-  rc = R && V ? cudaFuncSetAttribute(append_kernel<T, EL, V, R>, cudaFuncAttributeMaxDynamicSharedMemorySize,  \
+  rc = R && V ? cudaFuncSetAttribute(append_kernel<T, EL, ROWS, V, R>, cudaFuncAttributeMaxDynamicSharedMemorySize,  \
                                      (int)cfg.dynamicSmemBytes)                                               \
               : cudaSuccess;                                                                                  \
-  if (rc == cudaSuccess) rc = cudaLaunchKernelEx(&cfg, append_kernel<T, EL, V, R>, p, ra, (unsigned)n_append, (unsigned)groups)
+  if (rc == cudaSuccess)                                                                                      \
+    rc = cudaLaunchKernelEx(&cfg, append_kernel<T, EL, ROWS, V, R>, p, ra, (unsigned)n_append, (unsigned)groups)
   if (c->head_dim == 128) {
     if (rope) {
       if (vec) { GO(4, true, true); }
@@ -910,6 +935,14 @@ int launch_append(AppendArgs& p, const hc_rope_args* rope, const hc_kv_pages* c,
   }
 #undef GO
   return rc == cudaSuccess ? HC_OK : HC_ERR_CUDA;
+}
+
+int launch_append(AppendArgs& p, int dtype, const hc_rope_args* rope, const hc_kv_pages* c, cudaStream_t stream) {
+  if (p.n_rows < SPLIT_ROWS)
+    return dtype == HC_F16 ? launch_append<__half, FEW>(p, rope, c, stream)
+                           : launch_append<__nv_bfloat16, FEW>(p, rope, c, stream);
+  return dtype == HC_F16 ? launch_append<__half, MANY>(p, rope, c, stream)
+                         : launch_append<__nv_bfloat16, MANY>(p, rope, c, stream);
 }
 
 AppendArgs append_args(const hc_kv_pages* c, const void* k, int64_t k_row, int64_t k_head, const void* v,
@@ -1005,8 +1038,7 @@ extern "C" int hc_kv_append(const hc_kv_pages* cache, const void* k, int64_t k_r
   if (n_rows == 0) return HC_OK;
   AppendArgs p = append_args(cache, k, k_row, k_head, v, v_row, v_head, slots, n_rows, status);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return dtype == HC_F16 ? launch_append<__half>(p, nullptr, cache, s)
-                         : launch_append<__nv_bfloat16>(p, nullptr, cache, s);
+  return launch_append(p, dtype, nullptr, cache, s);
 }
 
 extern "C" int hc_rope_append(const hc_rope_args* a, const hc_kv_pages* cache, const void* v, int64_t v_row,
@@ -1026,5 +1058,5 @@ extern "C" int hc_rope_append(const hc_rope_args* a, const hc_kv_pages* cache, c
   p.rot = a->rotary_dim;
   p.interleaved = a->interleaved;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return a->dtype == HC_F16 ? launch_append<__half>(p, a, cache, s) : launch_append<__nv_bfloat16>(p, a, cache, s);
+  return launch_append(p, a->dtype, a, cache, s);
 }
