@@ -626,7 +626,7 @@ extern "C" int hc_paged_attn(const hc_attn_args* a, const hc_kv_pages* c, void* 
   if (!c->k || !c->v || !c->k_scale || !c->v_scale || c->n_pages <= 0 || c->n_kv_heads <= 0) return HC_ERR_ARG;
   if (a->n_requests <= 0 || a->n_rows < 0 || a->max_q < 0 || a->n_q_heads <= 0 ||
       a->n_q_heads % c->n_kv_heads || a->table_width <= 0 || a->table_stride < a->table_width ||
-      (a->dtype != HC_F16 && a->dtype != HC_BF16))
+      (a->dtype != HC_F16 && a->dtype != HC_BF16) || !(fabsf(a->scale) < INFINITY))
     return HC_ERR_ARG;
   if (a->q_row < 0 || a->q_head < 0 || a->out_row < 0 || a->out_head < 0) return HC_ERR_ARG;
   if (!aligned(a->q, 2) || !aligned(a->out, 2) || !aligned(a->lse, 4) || !aligned(c->k, 16) || !aligned(c->v, 16) ||

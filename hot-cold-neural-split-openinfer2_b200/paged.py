@@ -33,6 +33,7 @@ import hc_native as N
 
 _DTYPES = {torch.float16: N.HC_F16, torch.bfloat16: N.HC_BF16}
 PAGE_SIZES = (16, 32, 64, 128)
+MAX_REQUESTS = 2048             # of one call
 
 
 # ─── Argument checks ──────────────────────────────────────────────────────────
@@ -161,7 +162,7 @@ def rope_frequencies(rotary_dim: int, theta: float, scaling: Optional[dict] = No
     "dynamic" (base raised for ``max_seq_len`` beyond the original length);
     "yarn" (long wavelengths divided, short ones kept, a linear ramp between
     ``beta_fast`` and ``beta_slow`` turns over the original length, and the
-    attention factor); "llama3" (the ramp between ``high_freq_factor`` and
+    attention factor: given, or from ``mscale`` and ``mscale_all_dim``); "llama3" (the ramp between ``high_freq_factor`` and
     ``low_freq_factor`` wavelengths of the original length)."""
     _need(rotary_dim > 0 and rotary_dim % 2 == 0, "rotary_dim must be even and positive")
     half = rotary_dim // 2
@@ -176,6 +177,7 @@ def rope_frequencies(rotary_dim: int, theta: float, scaling: Optional[dict] = No
     original = scaling.get("original_max_position_embeddings")
     _need(original is not None and original > 0, f"{kind} scaling needs original_max_position_embeddings")
     if kind == "dynamic":
+        _need(rotary_dim > 2, "dynamic scaling needs more than one pair")
         length = max(int(max_seq_len), int(original))
         base *= (factor * length / original - (factor - 1)) ** (rotary_dim / (rotary_dim - 2))
         return base ** (-i / half), 1.0
@@ -183,12 +185,17 @@ def rope_frequencies(rotary_dim: int, theta: float, scaling: Optional[dict] = No
     if kind == "yarn":
         def pair(turns):           # the pair that makes so many turns over the original length
             return half * math.log(original / (turns * 2 * math.pi)) / math.log(base)
-        low = max(math.floor(pair(float(scaling.get("beta_fast", 32)))), 0)
-        high = min(math.ceil(pair(float(scaling.get("beta_slow", 1)))), rotary_dim - 1)
+        low, high = pair(float(scaling.get("beta_fast", 32))), pair(float(scaling.get("beta_slow", 1)))
+        if scaling.get("truncate", True):
+            low, high = math.floor(low), math.ceil(high)
+        low, high = max(low, 0), min(high, rotary_dim - 1)
         ramp = ((i - low) / max(high - low, 0.001)).clamp(0, 1)       # 0: kept, 1: divided
         attention = scaling.get("attention_factor")
         if attention is None:
-            attention = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+            def temper(weight):
+                return 0.1 * weight * math.log(factor) + 1.0 if factor > 1 else 1.0
+            every = scaling.get("mscale_all_dim")                     # given: the model's scale has this part already
+            attention = temper(float(scaling.get("mscale") or 1)) / (temper(float(every)) if every else 1.0)
         return freq * (1 - ramp) + freq / factor * ramp, float(attention)
     if kind == "llama3":
         lo, hi = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
@@ -237,7 +244,8 @@ def rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
     ``cos`` / ``sin`` [positions, rotary_dim // 2] fp32; pairs are (i, i +
     rotary_dim / 2), or (2i, 2i + 1) when ``interleaved``; dims past rotary_dim
     pass through.  Returns (q_out, k_out), new tensors unless given (q and k
-    themselves rotate in place).  Rows at position -1 are left alone."""
+    themselves rotate in place; outputs must not overlap the inputs otherwise).
+    Rows at position -1 are left alone."""
     if q_out is None:
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if k_out is None:
@@ -291,7 +299,7 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Te
                 k_scale: torch.Tensor, v_scale: torch.Tensor, *, interleaved: bool = False,
                 q_out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """:func:`rope` of q and k and :func:`kv_append` of the rotated k and of v
-    in one launch (hc_rope_append), with the same results.  Returns q_out."""
+    in one call (hc_rope_append), with the same results.  Returns q_out."""
     if q_out is None:
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     args = _rope_args(q, k, q_out, k, cos, sin, positions, interleaved)
@@ -322,7 +330,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     chooses the kernels, any value gives right results.  ``scale`` defaults to
     dim ** -0.5.  ``lse`` (optional, [rows, heads] fp32) receives the logarithm
     of each softmax's sum.  A row that sees no key gives 0 and -inf; padding
-    rows of ``out`` are left as they were."""
+    rows of ``out`` are left as they were.  ``out`` may be ``q`` itself, but not
+    overlap it otherwise."""
     pages = _pages(k_pages, v_pages, k_scale, v_scale)
     qp, dev = _heads(q, "q"), k_pages.get_device()
     rows, heads, dim = q.shape
@@ -363,6 +372,7 @@ class PagedKVCache:
                  max_requests: int = 64, max_len: int = 8192, device="cuda"):
         _need(page_size in PAGE_SIZES, f"page_size must be one of {PAGE_SIZES}")
         _need(head_dim in (64, 128), "head_dim must be 64 or 128")
+        _need(max_requests <= MAX_REQUESTS, f"max_requests must be at most {MAX_REQUESTS}")
         _need(n_layers > 0 and n_kv > 0 and n_pages > 0 and max_requests > 0 and max_len > 0, "sizes must be positive")
         self.page_size, self.max_requests = page_size, max_requests
         self.k = torch.zeros(n_layers, n_pages, n_kv, page_size, head_dim, dtype=torch.uint8, device=device)

@@ -604,8 +604,8 @@ HC_API int hc_page_release(const uint8_t* done, int32_t n_requests, int32_t* tab
 typedef struct hc_rope_args {
   const void* q;
   const void* k;
-  void* q_out;                      /* may be q */
-  void* k_out;                      /* may be k; not used by hc_rope_append */
+  void* q_out;                      /* may be q (same strides), else must not overlap the inputs */
+  void* k_out;                      /* likewise for k; not used by hc_rope_append */
   int64_t q_row, q_head, k_row, k_head;
   int64_t q_out_row, q_out_head, k_out_row, k_out_head;
   const float* cos_t;               /* [table_rows][rotary_dim / 2] fp32 */
@@ -647,8 +647,8 @@ HC_API int hc_kv_append(const hc_kv_pages* cache, const void* k, int64_t k_row, 
 
 /*
  * hc_rope_append -- hc_rope on q (into q_out) and on k, and hc_kv_append of
- * the rotated k (rounded to dtype first) and of v, in one launch: the same
- * bytes as the two calls.
+ * the rotated k (rounded to dtype first) and of v, in one launch (two from
+ * 1024 rows on): the same bytes as the two calls.
  */
 HC_API int hc_rope_append(const hc_rope_args* args, const hc_kv_pages* cache, const void* v, int64_t v_row,
                           int64_t v_head, const int64_t* slots, int32_t* status, hc_stream_t stream);
@@ -660,15 +660,17 @@ HC_API int hc_rope_append(const hc_rope_args* args, const hc_kv_pages* cache, co
  * pos counted so that its last row sits at kv_lens[r] - 1; query head h reads
  * key-value head h / (n_q_heads / n_kv_heads).
  *   q, out     [n_rows] rows of n_q_heads heads of head_dim (HC_F16 or
- *              HC_BF16), strided in elements
+ *              HC_BF16), strided in elements (strides not negative); out may
+ *              be q with its strides, else must not overlap it
+ *   scale      of the scores, finite (else HC_ERR_ARG)
  *   lse        optional [n_rows][n_q_heads] fp32: log of the softmax's sum
  *              (natural logarithm of sum exp(scale q k)); -inf for a row that
  *              sees nothing, whose output is 0
  *   tables, table_stride, table_width, cu_q, kv_lens  as in hc_page_plan
  *   max_q      host: the largest q_lens (chooses the kernels; any value is
  *              answered correctly)
- *   workspace  hc_paged_attn_workspace_bytes(...) bytes, 16-byte aligned
- *              (scratch; no initial contents needed; not shared by calls that
+ *   workspace  hc_paged_attn_workspace_bytes(...) bytes, 16-byte aligned, for
+ *              these n_requests, n_rows and heads (scratch; no initial contents needed; not shared by calls that
  *              can overlap)
  * Softmax statistics are fp32; a page id outside the cache, a length past the
  * table or rows past n_rows set HC_ERR_RANGE and are left out.  Bytes of

@@ -694,3 +694,153 @@ def test_serving_steps_in_a_graph_on_another_stream(P, N):
         for _ in range(3):
             run(graph=graph, res=res)
     torch.cuda.current_stream().wait_stream(side)
+
+
+# ─── sizes at which a call takes another way ──────────────────────────────────
+@pytest.mark.parametrize("rows_each,requests,page,dim,nkv", [
+    (1, 1100, 16, 128, 2), (1, 600, 64, 64, 1), (3, 400, 32, 128, 1), (1, 20, 128, 128, 5), (17, 70, 16, 64, 3),
+])
+def test_kv_append_many_short_runs(P, N, rows_each, requests, page, dim, nkv):
+    """A decode step of many requests: every run enters a page that holds tokens already, or begins one."""
+    g = _gen(rows_each + requests)
+    n_pages = requests * 2 + 3
+    at = torch.randint(0, page, (requests, 1), generator=g, device="cuda") + torch.arange(rows_each, device="cuda")
+    order = torch.randperm(n_pages, generator=g, device="cuda")[:2 * requests].view(requests, 2)
+    slots = (order.gather(1, at // page) * page + at % page).view(-1)
+    slots[rows_each * 5:rows_each * 6] = -1
+    cache = _cache(n_pages, nkv, page, dim, seed=requests)
+    before = _np(*cache)
+    kv = torch.randn(slots.numel(), 2 * nkv, dim, generator=g, device="cuda")
+    kv = (kv * 10.0 ** torch.randint(-3, 3, (slots.numel(), 1, 1), generator=g, device="cuda")).half()
+    st = N.new_status("cuda")
+    P.kv_append(kv[:, :nkv], kv[:, nkv:], slots, *cache, status=st)
+    N.read_status(st, "kv_append")
+    _check_append(cache, before, kv[:, :nkv], kv[:, nkv:], slots)
+
+
+@pytest.mark.parametrize("lens,page", [((500,), 32), ((1023, 0), 64), ((700, 324), 16), ((1, 1500, 800), 128),
+                                       ((33,) * 40, 64)])
+@pytest.mark.parametrize("dim,rotary,interleaved,aligned", [(128, 128, False, True), (128, 64, True, True),
+                                                            (64, 64, False, True), (64, 22, False, False)])
+def test_rope_append_of_prompts_is_rope_then_append(P, N, lens, page, dim, rotary, interleaved, aligned):
+    nq, nkv, g = 4, 2, _gen(sum(lens) + dim)
+    spans = [((7 * r) % 50, n) for r, n in enumerate(lens)]
+    pos = torch.cat([torch.arange(s, s + n, device="cuda") for s, n in spans] + [_i64([-1] * 3)])
+    wide = -(-max(s + n for s, n in spans) // page) * page
+    slots = torch.cat([torch.arange(s, s + n, device="cuda") + wide * r for r, (s, n) in enumerate(spans)]
+                      + [_i64([-1] * 3)])
+    rows = pos.numel()
+    cos, sin = _angles(P, 1600, rotary)
+    qkv = torch.randn(rows, (nq + 2 * nkv) * dim + 1, generator=g, device="cuda").half()
+    qkv = (qkv[:, :-1].contiguous() if aligned else qkv[:, 1:]).unflatten(1, (nq + 2 * nkv, dim))
+    q, k, v = qkv[:, :nq], qkv[:, nq:nq + nkv], qkv[:, nq + nkv:]
+    n_pages = len(lens) * wide // page
+    a, b = _cache(n_pages, nkv, page, dim, seed=2), _cache(n_pages, nkv, page, dim, seed=2)
+    st = N.new_status("cuda")
+    before = _np(*a)
+    k1 = torch.zeros_like(k, memory_format=torch.contiguous_format)
+    q1, _ = P.rope(q, k, cos, sin, pos, interleaved=interleaved, k_out=k1, status=st)
+    P.kv_append(k1, v, slots, *a, status=st)
+    _check_append(a, before, k1, v, slots)
+    q2 = torch.full_like(q1, 3.0)
+    P.rope_append(q, k, v, cos, sin, pos, slots, *b, interleaved=interleaved, q_out=q2, status=st)
+    N.read_status(st, "rope_append")
+    assert torch.equal(q1[:-3], q2[:-3]) and (q2[-3:] == 3).all()
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("requests", [33, 257, 2048])
+def test_paged_attention_many_requests(P, N, requests):
+    """More requests than a kernel keeps the lengths of; some without keys, some with many rows."""
+    page, nq, nkv, dim = 16, 8, 2, 64
+    g = _gen(requests)
+    spans = [(1 + (13 * r) % 40, (1 + r % 3) if r % 7 else 0) for r in range(requests)]
+    spans = [(max(kv, n), n) for kv, n in spans]
+    spans[requests // 2] = (90, 70)                  # several tiles
+    spans[-1] = (50, 9)
+    spans[3] = (0, 0)
+    tables, cu, kv, n_pages = _step(spans, page, g)
+    cache = _filled(n_pages, nkv, page, dim, g)
+    rows = int(cu[-1])
+    q = torch.randn(rows + 1, nq, dim, generator=g, device="cuda").half()
+    st = N.new_status("cuda")
+    for max_q in (1, 70):
+        out, lse = torch.full_like(q, 9.0), torch.full((rows + 1, nq), 9.0, device="cuda")
+        P.paged_attention(q, *cache, tables, cu, kv, max_q=max_q, out=out, lse=lse, status=st)
+        N.read_status(st, "paged_attention")
+        assert (out[rows] == 9).all()
+        _check_attention(out, lse, q, cache, tables, cu, kv)
+
+
+@pytest.mark.parametrize("spans", [[(300, 1), (5, 1), (9000, 1)], [(300, 200), (40, 1)], [(6000, 50)]])
+def test_paged_attention_over_its_queries_and_any_scale(P, N, spans):
+    page, nq, nkv, dim = 64, 8, 2, 128
+    g = _gen(len(spans))
+    tables, cu, kv, n_pages = _step(spans, page, g)
+    cache = _filled(n_pages, nkv, page, dim, g)
+    q = torch.randn(int(cu[-1]), nq, dim, generator=g, device="cuda").half()
+    m = max(n for _, n in spans)
+    want = P.paged_attention(q, *cache, tables, cu, kv, max_q=m)
+    inplace = q.clone()
+    assert P.paged_attention(inplace, *cache, tables, cu, kv, max_q=m, out=inplace) is inplace
+    assert torch.equal(inplace, want)
+    for scale in (0.0, -0.07):                       # the mean of the values; signs turned
+        out = P.paged_attention(q, *cache, tables, cu, kv, max_q=m, scale=scale)
+        _check_attention(out, None, q, cache, tables, cu, kv, scale=scale)
+    with pytest.raises(N.HotColdError):
+        P.paged_attention(q, *cache, tables, cu, kv, max_q=m, scale=float("nan"))
+
+
+def test_two_graphs_replayed_beside_each_other(P, N):
+    """Two captured calls hold a workspace each: they may run at once."""
+    page, nq, nkv, dim = 64, 8, 2, 128
+    g = _gen(77)
+    sides = []
+    for spans in ([(7000, 1), (300, 1)], [(5000, 40), (9000, 1)]):
+        tables, cu, kv, n_pages = _step(spans, page, g)
+        cache = _filled(n_pages, nkv, page, dim, g)
+        q = torch.randn(int(cu[-1]), nq, dim, generator=g, device="cuda").half()
+        m = max(n for _, n in spans)
+        want = P.paged_attention(q, *cache, tables, cu, kv, max_q=m)
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            out = P.paged_attention(q, *cache, tables, cu, kv, max_q=m)
+        sides.append((stream, graph, out, want, (q, cache, tables, cu, kv)))
+    for _ in range(30):
+        for stream, graph, *_ in sides:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, _, out, want, _ in sides:
+        assert torch.equal(out, want)
+
+
+def test_paged_cache_object(P, N):
+    """plan, append, attend, commit, release and check as methods, over two layers of one table."""
+    c = P.PagedKVCache(2, 2, 64, 7, page_size=16, max_requests=3, max_len=64)
+    assert len(c) == 2 and c.tables.shape == (3, 4) and [t.shape[0] for t in c[1]] == [7] * 4
+    g = _gen(5)
+    q_lens = _i32([20, 0, 30])
+    plan = c.plan(q_lens, 52)
+    kv = torch.randn(2, 2, 52, 2, 64, generator=g, device="cuda").half()
+    q = torch.randn(52, 4, 64, generator=g, device="cuda").half()
+    for layer in range(2):
+        before = _np(*c[layer])
+        c.append(layer, kv[layer, 0], kv[layer, 1], plan)
+        _check_append(c[layer], before, kv[layer, 0], kv[layer, 1], plan.slots)
+        out = torch.zeros_like(q)
+        c.attend(layer, q, plan, max_q=30, out=out)
+        _check_attention(out, None, q, c[layer], c.tables, plan.cu_q, plan.kv_lens)
+    c.commit(plan)
+    c.check()
+    assert c.lens.tolist() == [20, 0, 30] and int(c.n_free) == 3
+    c.release(torch.tensor([False, False, True], device="cuda"))
+    assert c.lens.tolist() == [20, 0, 0] and int(c.n_free) == 5 and (c.tables[2] == -1).all()
+    plan = c.plan(_i32([0, 0, 64]), 64)
+    assert int(c.n_free) == 1
+    c.check()
+    plan = c.plan(_i32([0, 40, 64]), 104)            # more pages than are left: nothing is taken
+    assert int(c.n_free) == 1 and (plan.slots == -1).all()
+    with pytest.raises(N.HotColdError):
+        c.check()

@@ -186,3 +186,36 @@ def test_oracle_e4m3_against_torch():
     x = torch.cat([x.clamp(-448, 448), mid, -mid])
     assert np.array_equal(O.e4m3_encode(x.double().numpy()), x.to(torch.float8_e4m3fn).view(torch.uint8).numpy())
     assert O.page_scale(448.0) == 1.0 and O.page_scale(448.0001) == 2.0 and O.page_scale(0.0) == 2.0 ** -40
+
+
+def test_yarn_attention_factor_and_ramp():
+    import paged
+    y = {"rope_type": "yarn", "factor": 40.0, "original_max_position_embeddings": 4096, "mscale": 1.0}
+    t = 0.1 * math.log(40) + 1
+    assert abs(paged.rope_frequencies(64, 1e4, y)[1] - t) < 1e-12
+    y["mscale_all_dim"] = 0.707
+    assert abs(paged.rope_frequencies(64, 1e4, y)[1] - t / (0.0707 * math.log(40) + 1)) < 1e-12
+    assert paged.rope_frequencies(64, 1e4, dict(y, mscale_all_dim=1.0))[1] == 1.0
+    assert paged.rope_frequencies(64, 1e4, dict(y, attention_factor=1.5))[1] == 1.5
+    # without rounding of the ramp's ends: the pair that turns 32 times is kept, the one that turns once divided
+    f, _ = paged.rope_frequencies(64, 1e4, dict(y, truncate=False))
+    freq = np.array([1e4 ** (-i / 32) for i in range(32)])
+    end = [32 * math.log(4096 / (n * 2 * math.pi)) / math.log(1e4) for n in (32, 1)]
+    ramp = np.clip((np.arange(32) - end[0]) / (end[1] - end[0]), 0, 1)
+    assert np.allclose(f.numpy(), freq * (1 - ramp) + freq / 40 * ramp, rtol=1e-12)
+
+
+def test_paged_refusals_of_scales_and_sizes(N):
+    import paged
+    c = _pages(N)
+    for scale in (float("nan"), float("inf"), -float("inf")):
+        assert N.lib.hc_paged_attn(ctypes.byref(_attn(N, scale=scale)), ctypes.byref(c), FAKE, 1 << 30, None,
+                                   None) == N.HC_ERR_ARG
+    with pytest.raises(ValueError):
+        paged.rope_frequencies(2, 1e4, {"rope_type": "dynamic", "factor": 2.0,
+                                        "original_max_position_embeddings": 64}, 128)
+    for bad in ({"page_size": 24}, {"max_requests": 2049}, {"max_len": 0}):
+        with pytest.raises(ValueError):
+            paged.PagedKVCache(1, 1, 64, 4, device="cpu", **bad)
+    with pytest.raises(ValueError):
+        paged.PagedKVCache(1, 1, 96, 4, device="cpu")
