@@ -17,6 +17,12 @@
 // value scale costs nothing and p (rounded to f16 for the product: relative
 // 2^-11, like the output) is as large as the running maximum allows.  m moves
 // only when a score passes it by 2^8, which f16 holds easily.
+//
+// Bound by HBM, each cached byte read once: 4 requests of 60,000 to 131,000
+// keys, 32 / 8 heads of 128, 134 us (5.8 TB/s; a copy of this loop that only
+// loads takes 132); 64 requests of 100 to 8000 keys 96 us (5.6 TB/s).  Three
+// CTAs of four warps on an SM; two, eight warps each, were slower, and so were
+// shares of a half or a quarter of this length (more items are cut).
 #include "hc_paged_attn.cuh"
 
 namespace hca8 {
@@ -26,7 +32,9 @@ constexpr int THREADS = 128;
 constexpr int WARPS = THREADS / 32;
 constexpr int STAGES = 3;              // chunks in flight per warp
 constexpr int ITEM_COST = 16;          // what beginning an item costs, in chunks
-constexpr int SMALL = 16;              // rows of a request and head that these kernels take
+// Rows of a request and head that these kernels take: two MMA columns of 8.  64 requests of 100 to 8000 keys with
+// 16 rows take 129 us here; with 20 rows the tiles of hc_paged_prefill.cu take 274 us, and as much for fewer.
+constexpr int SMALL = 16;
 constexpr int MIN_SHARE = 2 * WARPS;   // units of a share at least
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
@@ -500,7 +508,8 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) paged_attn_kernel(co
 
 // Joins the pieces of the items that the shares' borders divide, in the order
 // of the shares: two rows a CTA, 32 lanes of four dims each, the pieces dealt
-// to groups of lanes whose sums meet in shared memory.
+// to groups of lanes whose sums meet in shared memory.  Launched ahead of the
+// pieces' end; it adds 1 to 2 us, all of it latency.
 constexpr int JOIN_ROWS = 2;
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(THREADS) paged_join_kernel(const AttnParams p) {
@@ -510,7 +519,8 @@ __global__ void __launch_bounds__(THREADS) paged_join_kernel(const AttnParams p)
   __shared__ float s_acc[GROUPS][JOIN_ROWS][LANES][6];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int cta = blockIdx.x;
-  const int4 cut = p.cuts[2 * cta], rest = p.cuts[2 * cta + 1];      // request, head, first row, pieces; rows, first token
+  const int4 cut = p.cuts[2 * cta];             // request, head, first row, pieces
+  const int4 rest = p.cuts[2 * cta + 1];        // rows, first token
   const int n = cut.w;
   const int row = blockIdx.y * JOIN_ROWS + (threadIdx.x / LANES) % JOIN_ROWS, d = (threadIdx.x % LANES) * 4;
   if (n == 0 || blockIdx.y * JOIN_ROWS >= rest.x) return;
@@ -599,7 +609,7 @@ int launch(AttnParams& p, void* workspace, cudaStream_t stream) {
 
 template <typename T>
 int launch_typed(AttnParams& p, int head_dim, int rows, void* workspace, cudaStream_t stream) {
-  // rows of a request and head: 8 fill one MMA's columns, more take two
+  // rows of a request and head: 8 fill one MMA's columns (64 requests as above 99 us), more take two (128 us)
   if (head_dim == 128)
     return rows <= 8 ? launch<T, 128, 1>(p, workspace, stream) : launch<T, 128, 2>(p, workspace, stream);
   return rows <= 8 ? launch<T, 64, 1>(p, workspace, stream) : launch<T, 64, 2>(p, workspace, stream);
@@ -639,7 +649,8 @@ extern "C" int hc_paged_attn(const hc_attn_args* a, const hc_kv_pages* c, void* 
   if ((int64_t)a->table_width * c->page_size > INT32_MAX) return HC_ERR_ARG;
   if (a->n_rows == 0) return HC_OK;
   if (!workspace || !aligned(workspace, 16) ||
-      workspace_bytes < hc_paged_attn_workspace_bytes(a->n_requests, a->n_rows, a->n_q_heads, c->n_kv_heads, c->head_dim))
+      workspace_bytes <
+          hc_paged_attn_workspace_bytes(a->n_requests, a->n_rows, a->n_q_heads, c->n_kv_heads, c->head_dim))
     return HC_ERR_ARG;
   AttnParams p = {};
   p.q = a->q;
