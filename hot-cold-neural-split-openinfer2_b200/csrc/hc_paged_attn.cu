@@ -647,6 +647,7 @@ extern "C" int hc_paged_attn(const hc_attn_args* a, const hc_kv_pages* c, void* 
   if ((c->head_dim != 64 && c->head_dim != 128) || a->n_q_heads / c->n_kv_heads > 16 || a->n_requests > MAX_REQ)
     return HC_ERR_UNSUPPORTED;
   if ((int64_t)a->table_width * c->page_size > INT32_MAX) return HC_ERR_ARG;
+  if ((int64_t)a->n_rows * (a->n_q_heads / c->n_kv_heads) > 1 << 30) return HC_ERR_UNSUPPORTED;   // rows are int32
   if (a->n_rows == 0) return HC_OK;
   if (!workspace || !aligned(workspace, 16) ||
       workspace_bytes <

@@ -328,7 +328,14 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
     __syncthreads();
   }
   const int piece = s_piece, all = s_pre[p.n_req].x;
-  if (blockIdx.x == 0 && t == 0) p.pf_cuts[0] = make_int4(s_pre[p.n_req].y, 0, 0, 0);
+  // Offsets that go back and forth (each request in range by itself) claim more rows than there are: the grid would
+  // leave pieces out and the join would read slots that nothing wrote.  None of them is served then.
+  const bool over = (unsigned)all > gridDim.x;
+  if (blockIdx.x == 0 && t == 0) {
+    p.pf_cuts[0] = make_int4(over ? 0 : s_pre[p.n_req].y, 0, 0, 0);
+    if (over && p.status) atomicOr(p.status, HC_ERR_RANGE);
+  }
+  if (over) return;
   // later tiles see more keys: they start first
   const int unit = all - 1 - (int)blockIdx.x;
   if (unit < 0) return;

@@ -633,6 +633,8 @@ HC_API int hc_rope(const hc_rope_args* args, int32_t* status, hc_stream_t stream
  * distinct, and rows that enter one page follow one another in slot order
  * (as hc_page_plan gives them); a row that does not follow its predecessor
  * inside the same page sets HC_ERR_RANGE and is left out.
+ * (Two runs of one call that enter the same page, other rows between them, are
+ * not looked for: what that page then holds is not defined.)
  * The scale of a page and head is the smallest power of two 2^e, -40 <= e <=
  * 40, with |x| <= 448 * 2^e for its finite values.  Rows that begin a page
  * (its first slot among them) begin it anew; rows that enter it later raise
@@ -675,7 +677,11 @@ HC_API int hc_rope_append(const hc_rope_args* args, const hc_kv_pages* cache, co
  * Softmax statistics are fp32; a page id outside the cache, a length past the
  * table or rows past n_rows set HC_ERR_RANGE and are left out.  Bytes of
  * positions behind kv_lens are never used, whatever they hold.
- * n_requests <= 2048, n_q_heads / n_kv_heads <= 16 (else HC_ERR_UNSUPPORTED).
+ * A request whose offsets go back is left out with HC_ERR_RANGE, too; when
+ * such offsets make the others claim more rows than n_rows, those of more than
+ * 16 rows a key-value head may be left out as well.
+ * n_requests <= 2048, n_q_heads / n_kv_heads <= 16, n_rows times that ratio <=
+ * 2^30 (else HC_ERR_UNSUPPORTED).
  */
 typedef struct hc_attn_args {
   const void* q;

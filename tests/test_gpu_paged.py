@@ -844,3 +844,23 @@ def test_paged_cache_object(P, N):
     assert int(c.n_free) == 1 and (plan.slots == -1).all()
     with pytest.raises(N.HotColdError):
         c.check()
+
+
+@pytest.mark.parametrize("kv_len", [300, 6000])
+def test_paged_attention_offsets_that_go_back_and_forth(P, N, kv_len):
+    """Every other request claims the same rows: more tiles than the rows allow."""
+    page, nq, nkv, dim, n = 64, 8, 2, 64, 60
+    g = _gen(kv_len)
+    tables, _, _, n_pages = _step([(kv_len, 0)], page, g)
+    cache = _filled(n_pages, nkv, page, dim, g)
+    q = torch.randn(100, nq, dim, generator=g, device="cuda").half()
+    out, st = torch.full((101, nq, dim), 9.0, device="cuda").half(), N.new_status("cuda")
+    cu = _i32([0, 100] * (n // 2) + [0])
+    P.paged_attention(q, *cache, tables.expand(n, -1).contiguous(), cu, _i32([kv_len] * n), max_q=100, out=out[:100],
+                      status=st)
+    assert int(st) == N.HC_ERR_RANGE and (out[100] == 9).all()
+    good, st = _i32([0, 100]), N.new_status("cuda")        # the next call is none the worse
+    lens = _i32([kv_len])
+    got = P.paged_attention(q, *cache, tables, good, lens, max_q=100, status=st)
+    N.read_status(st, "paged_attention")
+    _check_attention(got, None, q, cache, tables, good, lens)

@@ -211,6 +211,8 @@ def test_paged_refusals_of_scales_and_sizes(N):
     for scale in (float("nan"), float("inf"), -float("inf")):
         assert N.lib.hc_paged_attn(ctypes.byref(_attn(N, scale=scale)), ctypes.byref(c), FAKE, 1 << 30, None,
                                    None) == N.HC_ERR_ARG
+    assert N.lib.hc_paged_attn(ctypes.byref(_attn(N, n_rows=(1 << 29) + 1)), ctypes.byref(c), FAKE, 1 << 30, None,
+                               None) == N.HC_ERR_UNSUPPORTED
     with pytest.raises(ValueError):
         paged.rope_frequencies(2, 1e4, {"rope_type": "dynamic", "factor": 2.0,
                                         "original_max_position_embeddings": 64}, 128)
