@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_release_kernel(const Releas
     for (int m = t; m < (int)total; m += PLAN_THREADS) {
       const int r = owner(s_put, p.n_req, m);
       const int32_t page = p.tables[r * p.stride + m - s_put[r]];
-      if (page >= p.n_pages) s_bad = 1;
+      if (page < 0 || page >= p.n_pages) s_bad = 1;      // a hole in a row, too
     }
   __syncthreads();
   if (over || s_bad) {                // more pages than there are: nothing is released

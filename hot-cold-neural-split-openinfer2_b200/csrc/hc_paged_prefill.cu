@@ -876,7 +876,8 @@ int launch_pf(AttnParams p, void* workspace, int sms, cudaStream_t stream) {
   if (pieces > INT32_MAX) return HC_ERR_UNSUPPORTED;
   paged_prefill_kernel<T, D><<<(unsigned)pieces, PF_THREADS, L::BYTES, stream>>>(p);
   if (cudaGetLastError() != cudaSuccess) return HC_ERR_CUDA;
-  if (((int64_t)p.width << p.page_log2) <= MIN_PIECE * HALF) return HC_OK;       // no length that the tables hold is cut
+  // no length that the tables hold is cut
+  if (((int64_t)p.width << p.page_log2) <= MIN_PIECE * HALF) return HC_OK;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(MAX_SMS / 2, D / 16);
   cfg.blockDim = dim3(ROWS);

@@ -162,8 +162,9 @@ def rope_frequencies(rotary_dim: int, theta: float, scaling: Optional[dict] = No
     "dynamic" (base raised for ``max_seq_len`` beyond the original length);
     "yarn" (long wavelengths divided, short ones kept, a linear ramp between
     ``beta_fast`` and ``beta_slow`` turns over the original length, and the
-    attention factor: given, or from ``mscale`` and ``mscale_all_dim``); "llama3" (the ramp between ``high_freq_factor`` and
-    ``low_freq_factor`` wavelengths of the original length)."""
+    attention factor: given, or from ``mscale`` and ``mscale_all_dim``);
+    "llama3" (the ramp between ``high_freq_factor`` and ``low_freq_factor``
+    wavelengths of the original length)."""
     _need(rotary_dim > 0 and rotary_dim % 2 == 0, "rotary_dim must be even and positive")
     half = rotary_dim // 2
     i = torch.arange(half, dtype=torch.float64, device=device)

@@ -864,3 +864,12 @@ def test_paged_attention_offsets_that_go_back_and_forth(P, N, kv_len):
     got = P.paged_attention(q, *cache, tables, good, lens, max_q=100, status=st)
     N.read_status(st, "paged_attention")
     _check_attention(got, None, q, cache, tables, good, lens)
+
+
+@pytest.mark.parametrize("row", [[3, -1, 5, 7], [3, 4, 9, -1], [3, -7, 5, 6]])
+def test_page_release_of_a_row_with_a_hole_or_a_stray_page(P, N, row):
+    tables, free, n_free, st = _i32([row, [1, 2, -1, -1]]), _i32([0] + [-1] * 8), _i32([1]), N.new_status("cuda")
+    before = tables.clone()
+    P.page_release(torch.tensor([True, True], device="cuda"), tables, free, n_free, st)
+    assert int(st) == N.HC_ERR_RANGE and int(n_free) == 1 and torch.equal(tables, before)
+    assert free.tolist() == [0] + [-1] * 8
