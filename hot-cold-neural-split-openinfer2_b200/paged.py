@@ -25,6 +25,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import struct
 from typing import NamedTuple, Optional
 
 import torch
@@ -41,6 +42,13 @@ MAX_REQUESTS = 2048             # of one call
 # is wrong is put into words only when one of them fails.
 _I32, _I64, _F32, _U8 = torch.int32, torch.int64, torch.float32, torch.uint8
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+# The argument structs as bytes: packing takes half of the time that building the ctypes structures does.
+_KV_PAGES, _ROPE_ARGS = struct.Struct("4P4i"), struct.Struct("4P8q2PqP7i0P")
+_ATTN_ARGS = struct.Struct("3P4qPqi2P4ifi0P")
+if (_KV_PAGES.size, _ROPE_ARGS.size, _ATTN_ARGS.size) != tuple(
+        ctypes.sizeof(c) for c in (N.KVPages, N.RopeArgs, N.AttnArgs)):
+    raise ImportError("the packed argument structs do not match hotcold.h")
 
 
 def _need(ok: bool, what: str):
@@ -92,8 +100,7 @@ def _status(t: Optional[torch.Tensor], dev: int) -> Optional[int]:
 
 def _call(fn, where: str, dev: int, *args):
     """fn(*args, stream) with ``dev`` current and its current stream."""
-    back = torch.cuda.current_device()
-    if back == dev:
+    if _current_device() == dev:
         rc = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
@@ -128,9 +135,9 @@ def page_plan(starts: torch.Tensor, q_lens: torch.Tensor, tables: torch.Tensor, 
     _need(n_rows >= 0, "n_rows must not be negative")
     device = starts.device
     cu_q = torch.empty(n + 1, dtype=_I32, device=device)
-    kv_lens = torch.empty(n, dtype=_I32, device=device)
+    kv_lens = torch.empty_like(starts)
     positions = torch.empty(n_rows, dtype=_I64, device=device)
-    slots = torch.empty(n_rows, dtype=_I64, device=device)
+    slots = torch.empty_like(positions)
     _call(N.lib.hc_page_plan, "hc_page_plan", dev, _vector(starts, "starts", _I32, None, dev),
           _vector(q_lens, "q_lens", _I32, n, dev), n, _table(tables, n, dev), tables.stride(0), tables.shape[1],
           _vector(free_pages, "free_pages", _I32, None, dev), free_pages.shape[0],
@@ -214,7 +221,7 @@ def rope_tables(max_seq_len: int, rotary_dim: int, theta: float, scaling: Option
     return (angle.cos() * factor).float(), (angle.sin() * factor).float()
 
 
-def _rope_args(q, k, q_out, k_out, cos, sin, positions, interleaved) -> N.RopeArgs:
+def _rope_args(q, k, q_out, k_out, cos, sin, positions, interleaved) -> bytes:
     qp, kp = _heads(q, "q"), _heads(k, "k", q)
     rows, nq, dim = q.shape
     dev = q.get_device()
@@ -232,9 +239,9 @@ def _rope_args(q, k, q_out, k_out, cos, sin, positions, interleaved) -> N.RopeAr
     k0, k1, _ = k.stride()
     r0, r1, _ = q_out.stride()
     t0, t1, _ = k_out.stride()
-    return N.RopeArgs(qp, kp, q_out.data_ptr(), k_out.data_ptr(), q0, q1, k0, k1, r0, r1, t0, t1, cp, sp, length,
-                      _vector(positions, "positions", _I64, rows, dev), rows, nq, k.shape[1], dim, 2 * half,
-                      1 if interleaved else 0, _DTYPES[q.dtype])
+    return _ROPE_ARGS.pack(qp, kp, q_out.data_ptr(), k_out.data_ptr(), q0, q1, k0, k1, r0, r1, t0, t1, cp, sp, length,
+                           _vector(positions, "positions", _I64, rows, dev), rows, nq, k.shape[1], dim, 2 * half,
+                           1 if interleaved else 0, _DTYPES[q.dtype])
 
 
 def rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor, *,
@@ -253,12 +260,12 @@ def rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
         k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
     args = _rope_args(q, k, q_out, k_out, cos, sin, positions, interleaved)
     dev = q.get_device()
-    _call(N.lib.hc_rope, "hc_rope", dev, ctypes.byref(args), _status(status, dev))
+    _call(N.lib.hc_rope, "hc_rope", dev, args, _status(status, dev))
     return q_out, k_out
 
 
 # ─── The cache: write and attention ───────────────────────────────────────────
-def _pages(k_pages, v_pages, k_scale, v_scale) -> N.KVPages:
+def _pages(k_pages, v_pages, k_scale, v_scale) -> bytes:
     dev = k_pages.get_device()
     if dev < 0:
         N.require_cuda(k_pages)
@@ -269,12 +276,13 @@ def _pages(k_pages, v_pages, k_scale, v_scale) -> N.KVPages:
             v_pages.get_device() != dev:
         _bad(v_pages, "v_pages", _U8, list(shape), dev)
     n, h, p, d = shape
-    return N.KVPages(k_pages.data_ptr(), v_pages.data_ptr(), _matrix(k_scale, "k_scale", _F32, n, h, dev),
-                     _matrix(v_scale, "v_scale", _F32, n, h, dev), n, h, p, d)
+    return _KV_PAGES.pack(k_pages.data_ptr(), v_pages.data_ptr(), _matrix(k_scale, "k_scale", _F32, n, h, dev),
+                          _matrix(v_scale, "v_scale", _F32, n, h, dev), n, h, p, d)
 
 
-def _fits(k: torch.Tensor, v: torch.Tensor, pages: N.KVPages, dev: int):
-    if k.shape != v.shape or k.shape[1] != pages.n_kv_heads or k.shape[2] != pages.head_dim or k.get_device() != dev:
+def _fits(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, dev: int):
+    pages = k_pages.shape
+    if k.shape != v.shape or k.shape[1] != pages[1] or k.shape[2] != pages[3] or k.get_device() != dev:
         raise ValueError("k and v must have the cache's heads, dim and device")
 
 
@@ -287,11 +295,11 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: to
     them); rows with a negative slot are padding."""
     pages = _pages(k_pages, v_pages, k_scale, v_scale)
     kp, vp, dev = _heads(k, "k"), _heads(v, "v", k), k_pages.get_device()
-    _fits(k, v, pages, dev)
+    _fits(k, v, k_pages, dev)
     k0, k1, _ = k.stride()
     v0, v1, _ = v.stride()
     rows = k.shape[0]
-    _call(N.lib.hc_kv_append, "hc_kv_append", dev, ctypes.byref(pages), kp, k0, k1, vp, v0, v1,
+    _call(N.lib.hc_kv_append, "hc_kv_append", dev, pages, kp, k0, k1, vp, v0, v1,
           _vector(slots, "slots", _I64, rows, dev), rows, _DTYPES[k.dtype], _status(status, dev))
 
 
@@ -306,9 +314,9 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Te
     args = _rope_args(q, k, q_out, k, cos, sin, positions, interleaved)
     pages = _pages(k_pages, v_pages, k_scale, v_scale)
     vp, dev = _heads(v, "v", k), k_pages.get_device()
-    _fits(k, v, pages, dev)
+    _fits(k, v, k_pages, dev)
     v0, v1, _ = v.stride()
-    _call(N.lib.hc_rope_append, "hc_rope_append", dev, ctypes.byref(args), ctypes.byref(pages), vp, v0, v1,
+    _call(N.lib.hc_rope_append, "hc_rope_append", dev, args, pages, vp, v0, v1,
           _vector(slots, "slots", _I64, k.shape[0], dev), _status(status, dev))
     return q_out
 
@@ -336,7 +344,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     pages = _pages(k_pages, v_pages, k_scale, v_scale)
     qp, dev = _heads(q, "q"), k_pages.get_device()
     rows, heads, dim = q.shape
-    if dim != pages.head_dim or q.get_device() != dev or heads % pages.n_kv_heads:
+    nkv = k_pages.shape[1]
+    if dim != k_pages.shape[3] or q.get_device() != dev or nkv == 0 or heads % nkv:
         raise ValueError("q must have the cache's dim and device, and a multiple of its heads")
     n = kv_lens.shape[0]
     if out is None:
@@ -347,13 +356,13 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         _need(out.shape[1] == heads, "out must have the shape of q")
     q0, q1, _ = q.stride()
     o0, o1, _ = out.stride()
-    args = N.AttnArgs(qp, op, None if lse is None else _matrix(lse, "lse", _F32, rows, heads, dev), q0, q1, o0, o1,
-                      _table(tables, n, dev), tables.stride(0), tables.shape[1],
-                      _vector(cu_q, "cu_q", _I32, n + 1, dev), _vector(kv_lens, "kv_lens", _I32, None, dev), n, rows,
-                      max_q, heads, dim ** -0.5 if scale is None else scale, _DTYPES[q.dtype])
-    need = max(_workspace_bytes(n, rows, heads, pages.n_kv_heads, dim), 16)
+    args = _ATTN_ARGS.pack(qp, op, 0 if lse is None else _matrix(lse, "lse", _F32, rows, heads, dev), q0, q1, o0, o1,
+                           _table(tables, n, dev), tables.stride(0), tables.shape[1],
+                           _vector(cu_q, "cu_q", _I32, n + 1, dev), _vector(kv_lens, "kv_lens", _I32, None, dev), n,
+                           rows, max_q, heads, dim ** -0.5 if scale is None else scale, _DTYPES[q.dtype])
+    need = max(_workspace_bytes(n, rows, heads, nkv, dim), 16)
     workspace = torch.empty(need, dtype=_U8, device=q.device)
-    _call(N.lib.hc_paged_attn, "hc_paged_attn", dev, ctypes.byref(args), ctypes.byref(pages), workspace.data_ptr(),
+    _call(N.lib.hc_paged_attn, "hc_paged_attn", dev, args, pages, workspace.data_ptr(),
           need, _status(status, dev))
     return out
 
