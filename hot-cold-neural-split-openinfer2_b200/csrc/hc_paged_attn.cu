@@ -14,9 +14,10 @@
 // where k_j, v_j are the raw e4m3 numbers (exact in f16).  In base 2, with
 // t_j = s_j log2(e) + log2(vs_j) and a running reference m: p_j = 2^{t_j - m}
 // is the weight of v_j and p_j / vs_j its share of the denominator, so the
-// value scale costs nothing and p (rounded to f16 for the product: relative
-// 2^-11, like the output) is as large as the running maximum allows.  m moves
-// only when a score passes it by 2^8, which f16 holds easily.
+// value scale costs nothing.  p is rounded to f16 for the product: relative
+// 2^-11, like the output, down to 2^-25 of the row's largest weight, and by
+// 2^-36 of that one at most below (W_REF in hc_paged_attn.cuh); a row of many
+// small weights beside one large one needs that room.
 //
 // Bound by HBM, each cached byte read once: 4 requests of 60,000 to 131,000
 // keys, 32 / 8 heads of 128, 134 us (5.8 TB/s; a copy of this loop that only
@@ -219,7 +220,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) paged_attn_kernel(co
       if (at != NONE) {
         const uint32_t head = at >> (p.page_log2 - 4);           // page * nkv + h
         a = __ldg(p.ks + head);
-        b = fmaxf(__ldg(p.vs + head), 1e-30f);
+        b = fmaxf(__ldg(p.vs + head), VS_MIN);
       }
       const float lb = __log2f(b), ib = __frcp_rn(b);
       if (set) sk[1] = a, sl[1] = lb, si[1] = ib;
@@ -372,7 +373,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) paged_attn_kernel(co
           float v = fmaf(s[nt][e] + s1[nt][e], fac[nt][e & 1] * kscale, lv);
           if (masked && key0 + i8 + (e >> 1) * 8 > lim[nt][e & 1]) v = -INFINITY;
           s[nt][e] = v;
-          over |= v > m[nt][e & 1] + 8.0f;
+          over |= v > m[nt][e & 1] + W_MAX;
         }
       if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
@@ -383,7 +384,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) paged_attn_kernel(co
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-            top = fmaxf(top, m[nt][e]);
+            top = fmaxf(top - W_REF, m[nt][e]);
             const float keep = ex2(m[nt][e] - top);
             m[nt][e] = top;
             l[nt][e] *= keep;

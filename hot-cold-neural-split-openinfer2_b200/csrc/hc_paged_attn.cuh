@@ -12,6 +12,13 @@ constexpr int MAX_REQ = 2048;
 constexpr uint32_t NONE = 0xffffffffu; // no page
 constexpr int KEPT_REQ = 256;          // requests whose lengths stay in shared memory
 constexpr float M_NONE = -1e30f;       // softmax reference before the first key
+// Weights are 2^(t - m), rounded to f16 for the product, and f16's step is 2^-24 at the bottom: the larger the
+// greatest weight, the smaller a weight may be beside it.  A row's reference m is put W_REF below its largest
+// exponent and moves when a weight would pass 2^W_MAX (65504 is the largest f16).  A weight of 2^-d of the largest
+// is then rounded by at most max(2^-11, 2^(d - 36)) of itself.  A window of 2^4 keeps moves rare: scores with a
+// deviation of 1 never leave it after the first keys.
+constexpr float W_REF = 11.0f, W_MAX = 15.0f;
+constexpr float VS_MIN = 0x1p-80f;     // value scales below count as this: 2^W_MAX / VS_MIN times 2^31 keys stays in fp32
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 

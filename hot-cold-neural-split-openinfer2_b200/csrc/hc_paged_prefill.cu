@@ -505,8 +505,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
         tmem_wait_ld(s[1]);
         if (masked) mask_row(s, last);
         const float top = row_max(s, sl, fac);
-        if (__any_sync(0xffffffffu, top > m + 8.0f)) {
-          const float m1 = fmaxf(m, top), keep = ex2(m - m1);
+        if (__any_sync(0xffffffffu, top > m + W_MAX)) {
+          const float m1 = fmaxf(m, top - W_REF), keep = ex2(m - m1);
           m = m1;
           l *= keep;
           if (i > 0) {
@@ -712,7 +712,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
     for (int j = 0; j < n_tiles; ++j) {
       Slice mine = {0.0f, -INFINITY, 0.0f};             // no page: no weight
       if ((unsigned)at < (unsigned)p.n_pages) {
-        const float b = fmaxf(vs, 1e-30f);
+        const float b = fmaxf(vs, VS_MIN);
         mine.k = ks;
         mine.lv = __log2f(b);
         mine.iv = __frcp_rn(b);

@@ -1,0 +1,74 @@
+"""The paged-cache operators where values, lengths or tables are at the edge of what they take.
+
+Oracle and helpers are those of test_gpu_paged.py; tolerances are derived at each test.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_paged import (HALF_STEP, N, P, _angles, _cache, _check_append, _check_attention, _filled, _gen, _i32,
+                            _i64, _np, _step)
+
+pytestmark = pytest.mark.gpu
+
+
+# ─── attention: weights far below the largest ─────────────────────────────────
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,dim,nats", [(1, 128, 17.0), (1, 64, 17.6), (3, 128, 17.6), (1, 128, 20.0),
+                                           (40, 128, 17.0), (40, 64, 17.6), (40, 128, 20.0)])
+def test_paged_attention_behind_a_sink(P, rows, dim, nats, dtype):
+    """One key of value 0 takes nearly all of the weight; 20,000 equal keys of value 1 share the rest.
+
+    With the sink at exponent d = nats log2(e), a weight beside it is rounded by max(2^-11, 2^(d - 36)) of itself
+    (weights are at least 2^(11 - d), f16's step at the bottom is 2^-24), all of them alike.  Sums of 20,000 keys in
+    fp32, 16 at a time, in the product and in the denominator, each step off by at most 2^-23: 2 * 1251 * 2^-23.
+    The scores, exponentials and the reciprocal: 2^-14, as in test_gpu_paged.py.  Then the output's half step, half of
+    f16's last step included."""
+    page, nkv, nq, n = 64, 1, 4, 20001
+    g = _gen(dim)
+    tables, cu, kv, n_pages = _step([(n + rows - 1, rows)], page, g)
+    kp = torch.zeros(n_pages, nkv, page, dim, dtype=torch.uint8, device="cuda")
+    vp = torch.full_like(kp, 0x38)                                     # 1.0
+    ks, vs = torch.ones(n_pages, nkv, device="cuda"), torch.ones(n_pages, nkv, device="cuda")
+    first = int(tables[0, 0])
+    kp[first, 0, 0, 0], vp[first, 0, 0] = 0x38, 0
+    q = torch.zeros(rows, nq, dim, device="cuda", dtype=dtype)
+    q[:, :, 0] = 1.0
+    out = P.paged_attention(q, kp, vp, ks, vs, tables, cu, kv, max_q=rows, scale=nats).double()
+    scale = float(np.float32(nats))
+    seen = torch.arange(n - 1, n - 1 + rows, dtype=torch.float64, device="cuda")        # keys beside the sink
+    want = (seen * math.exp(-scale) / (1 + seen * math.exp(-scale)))[:, None, None]
+    d = scale / math.log(2)
+    rel = max(2.0 ** -11, 2.0 ** (d - 36)) + 2 * 1251 * 2.0 ** -23 + 2.0 ** -14
+    tol = want * (rel + HALF_STEP[dtype]) * 1.01 + 2.0 ** -25
+    assert ((out - want).abs() <= tol).all(), ((out - want).abs() / want).max().item()
+
+
+@pytest.mark.parametrize("nq,nkv,dim,page,dtype", [(8, 2, 128, 64, torch.float16), (4, 1, 64, 16, torch.bfloat16)])
+@pytest.mark.parametrize("spans", [[(700, 1), (3000, 2)], [(500, 200), (2500, 40)]])
+@pytest.mark.parametrize("way", [1, -1])
+def test_paged_attention_scores_that_climb(P, spans, nq, nkv, dim, page, dtype, way):
+    """The largest score moves on with the keys (the reference is raised again and again, outputs and sums with it),
+    or stays behind at the first ones."""
+    g = _gen(nq + page)
+    tables, cu, kv, n_pages = _step(spans, page, g)
+    cache = _filled(n_pages, nkv, page, dim, g)
+    kp, _, ks, _ = cache
+    e4m3 = kp.view(torch.float8_e4m3fn)
+    for r, (n, _) in enumerate(spans):
+        pos = torch.arange(-(-n // page) * page, device="cuda").view(-1, page)
+        rise = (pos if way > 0 else n - pos).float() * (40.0 / n)       # score in nats that dimension 0 adds
+        ids = tables[r, :-(-n // page)].long()
+        ks[ids] = 1.0
+        x = torch.randn(len(ids), nkv, page, dim, generator=g, device="cuda")
+        x[..., 0] = rise[:, None]
+        e4m3[ids] = x.to(torch.float8_e4m3fn)
+    q = torch.randn(int(cu[-1]), nq, dim, generator=g, device="cuda") * 0.5
+    q[..., 0] = dim ** 0.5
+    q = q.to(dtype)
+    lse = torch.empty(q.shape[:2], device="cuda")
+    for m in (1, max(n for _, n in spans)):
+        out = P.paged_attention(q, *cache, tables, cu, kv, max_q=m, lse=lse)
+        _check_attention(out, lse, q, cache, tables, cu, kv)
