@@ -298,12 +298,15 @@ __device__ __forceinline__ T turn(T x, T y, float c, float s) {
 // rounded so.  The 16-bit value decides the byte that the cache holds, which
 // then depends on no order of operations.  Conversions to 64 bits and back run
 // at a sixteenth of the fp32 rate here, so this costs half of what they do.
+// Where fp32 does not hold the sum (or a product, under angles with a factor
+// above 1) it stands uncorrected, infinite or NaN as for queries: its error
+// terms are inf - inf.
 __device__ __forceinline__ float turn_exact(float x, float y, float c, float s) {
   const float p = __fmul_rn(x, c), q = __fmul_rn(y, s);
   const float e = __fmaf_rn(x, c, -p), f = __fmaf_rn(y, s, -q);
   const float r = __fadd_rn(p, q), z = __fsub_rn(r, p);
   const float t = __fadd_rn(__fsub_rn(p, __fsub_rn(r, z)), __fsub_rn(q, z));
-  return __fadd_rn(r, __fadd_rn(t, __fadd_rn(e, f)));
+  return fabsf(r) < INFINITY ? __fadd_rn(r, __fadd_rn(t, __fadd_rn(e, f))) : r;
 }
 template <typename T>
 __device__ __forceinline__ T turn_key(T x, T y, float c, float s) {

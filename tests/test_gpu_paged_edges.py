@@ -8,6 +8,7 @@ import numpy as np
 import pytest
 import torch
 
+import test_gpu_paged as T
 from test_gpu_paged import (HALF_STEP, N, P, _angles, _cache, _check_append, _check_attention, _filled, _gen, _i32,
                             _i64, _np, _step)
 
@@ -72,3 +73,50 @@ def test_paged_attention_scores_that_climb(P, spans, nq, nkv, dim, page, dtype, 
     for m in (1, max(n for _, n in spans)):
         out = P.paged_attention(q, *cache, tables, cu, kv, max_q=m, lse=lse)
         _check_attention(out, lse, q, cache, tables, cu, kv)
+
+
+# ─── keys that are not finite, or that the rotation makes so ──────────────────
+def _edge_rows(rows, heads, dim, dtype, g):
+    """Rows of ordinary values with infinities, NaN and pairs whose sums pass the type (and, in bf16, fp32)."""
+    x = torch.randn(rows, heads, dim, generator=g, device="cuda")
+    big = 65504.0 if dtype is torch.float16 else 3.3e38
+    inf = float("inf")
+    at = torch.randint(0, dim, (rows, heads, 2), generator=g, device="cuda")
+    what = torch.tensor([inf, -inf, float("nan"), big, -big, 1.0], device="cuda")
+    pick = what[torch.randint(0, 6, (rows, heads, 2), generator=g, device="cuda")]
+    x.scatter_(2, at, pick)
+    x[1::4] = big                            # every pair of the row at the top: a c - b s and a s + b c
+    x[3::4, :, ::2] = -big
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,dim,rotary,interleaved", [
+    (24, 128, 128, False), (24, 64, 32, True), (24, 64, 18, False), (1100, 128, 128, False), (1100, 64, 64, True),
+    (1100, 128, 30, True),
+])
+def test_keys_that_are_not_finite(P, N, rows, dim, rotary, interleaved, dtype):
+    """The rotation of infinities and of sums that overflow is the definition's (in 64 bits, rounded to fp32 and to
+    the type), and the cache holds them saturated at 448 times the scale, NaN as 0."""
+    nq, nkv, page = 4, 2, 64
+    g = _gen(rows + rotary)
+    cos, sin = _angles(P, 3000, rotary)
+    pos = torch.arange(rows, device="cuda")              # position 0 among them: sin is 0, and 0 times infinity NaN
+    k = _edge_rows(rows, nkv, dim, dtype, g)
+    v = torch.randn(rows, nkv, dim, generator=g, device="cuda").to(dtype)
+    q = torch.randn(rows, nq, dim, generator=g, device="cuda").to(dtype)
+    with np.errstate(invalid="ignore"):
+        want = T.O.rotate(k.double().cpu().numpy(), cos.double().cpu().numpy(), sin.double().cpu().numpy(),
+                          pos.tolist(), interleaved)
+    want = torch.from_numpy(want).float().to(dtype)
+    assert want.isinf().any() and want.isnan().any() and want[1::4].isinf().any()
+    got = P.rope(q, k, cos, sin, pos, interleaved=interleaved)[1].cpu()
+    lost = want.isnan()
+    assert torch.equal(got.isnan(), lost) and torch.equal(got.masked_fill(lost, 0), want.masked_fill(lost, 0))
+    n_pages = -(-rows // page)
+    cache = _cache(n_pages, nkv, page, dim, seed=3)
+    before = _np(*cache)
+    st = N.new_status("cuda")
+    P.rope_append(q, k, v, cos, sin, pos, pos, *cache, interleaved=interleaved, status=st)
+    assert int(st) == N.HC_ERR_RANGE
+    _check_append(cache, before, want.cuda(), v, pos)
