@@ -1295,7 +1295,9 @@ class DesdemonaEngine(nn.Module):
 
         ``q_lens[r]`` new tokens of request r follow its cached ones; ``tokens``
         [sum(q_lens)] holds them request after request.  All rows share one
-        fetch set per layer, as a batch does in the reference (engine.py:277)."""
+        fetch set per layer, as a batch does in the reference (engine.py:277).
+        A step that does not fit (too few free pages, a request past the
+        cache's ``max_len``) raises ValueError and leaves the cache as it was."""
         q_lens = [int(n) for n in q_lens]
         rows = sum(q_lens)
         if len(q_lens) > cache.max_requests or tokens.dim() != 1 or tokens.shape[0] != rows or rows == 0 or \
@@ -1303,10 +1305,22 @@ class DesdemonaEngine(nn.Module):
             raise ValueError("tokens must hold sum(q_lens) > 0 ids of at most max_requests requests")
         device_lens = torch.zeros(cache.max_requests, dtype=torch.int32)
         device_lens[:len(q_lens)] = torch.tensor(q_lens, dtype=torch.int32)
+        # The host waits for the plan's outcome while the first fetch set is predicted: no layer runs on rows that
+        # were not placed.
+        seen = torch.empty(2, dtype=torch.int32, pin_memory=True)        # status before the plan, rows placed
+        seen[:1].copy_(cache.status, non_blocking=True)
         plan = cache.plan(device_lens.to(self.device), rows)
+        seen[1:].copy_(plan.cu_q[-1:], non_blocking=True)
+        planned = torch.cuda.Event()
+        planned.record(torch.cuda.current_stream(self.device))
         x = self.embed_tokens(tokens.to(self.device))
         f, words, max_q = self.ffn_layers, self._words, max(q_lens)
         f[0].submit_cold_fetch(x.view(rows, 1, -1), out=words[0])
+        planned.synchronize()
+        if int(seen[1]) != rows:         # nothing was taken, every row is padding
+            cache.status.fill_(int(seen[0]))
+            raise ValueError(f"the step's {rows} tokens do not fit the cache: {int(cache.n_free)} pages are free, "
+                             f"requests hold up to {cache.max_len} positions")
         for li, att in enumerate(self.attention_layers):
             x = att.step_paged(x, self.cos_cache, self.sin_cache, cache, plan, max_q)
             if li + 1 < self.num_layers:

@@ -384,7 +384,7 @@ class PagedKVCache:
         _need(head_dim in (64, 128), "head_dim must be 64 or 128")
         _need(max_requests <= MAX_REQUESTS, f"max_requests must be at most {MAX_REQUESTS}")
         _need(n_layers > 0 and n_kv > 0 and n_pages > 0 and max_requests > 0 and max_len > 0, "sizes must be positive")
-        self.page_size, self.max_requests = page_size, max_requests
+        self.page_size, self.max_requests, self.max_len = page_size, max_requests, max_len
         self.k = torch.zeros(n_layers, n_pages, n_kv, page_size, head_dim, dtype=torch.uint8, device=device)
         self.v = torch.zeros_like(self.k)
         self.k_scale = torch.zeros(n_layers, n_pages, n_kv, device=device)

@@ -1,0 +1,49 @@
+"""The engine's paged steps that do not fit, and what generate_batch answers, checked from outside."""
+import pytest
+import torch
+
+from test_gpu_paged_engine import LOGIT_TOL, VOCAB, _Plain, _rel, make
+
+pytestmark = pytest.mark.gpu
+
+
+def _tokens(n, seed):
+    return torch.randint(0, VOCAB, (n,), generator=torch.Generator().manual_seed(seed)).cuda()
+
+
+def test_forward_paged_refuses_a_step_without_pages(make):
+    """Pages run out in the middle of a run: the step raises and takes nothing, and after a release it runs as if it
+    had not been tried."""
+    eng = make()
+    page = 16
+    cache, twin = (eng.new_paged_cache(2, n_pages=4, page_size=page, max_len=200) for _ in range(2))
+    a, b, c = _tokens(40, 1), _tokens(20, 2), _tokens(9, 3)
+    first = eng.forward_paged(a, [40, 0], cache)                       # 3 of 4 pages
+    assert _rel(first, eng.forward_paged(a, [40, 0], twin)) < LOGIT_TOL
+    state = [t.clone() for t in (cache.lens, cache.tables, cache.n_free, cache.k, cache.v, cache.k_scale)]
+    for _ in range(2):
+        with pytest.raises(ValueError, match="fit"):
+            eng.forward_paged(b, [0, 20], cache)
+    with pytest.raises(ValueError, match="fit"):
+        eng.forward_paged(torch.cat([c, b]), [9, 20], cache)           # neither request, though one would fit
+    now = (cache.lens, cache.tables, cache.n_free, cache.k, cache.v, cache.k_scale)
+    assert all(torch.equal(x, y) for x, y in zip(state, now))
+    cache.check()                                                      # reported by the exception already
+    assert _rel(eng.forward_paged(c, [9, 0], cache), eng.forward_paged(c, [9, 0], twin)) < LOGIT_TOL
+    done = torch.tensor([True, False], device="cuda")
+    cache.release(done)
+    twin.release(done)
+    assert _rel(eng.forward_paged(b, [0, 20], cache), eng.forward_paged(b, [0, 20], twin)) < LOGIT_TOL
+    cache.check()
+    eng.check()
+    # an error that was there before the refused step is still reported
+    cache.status.fill_(4)
+    with pytest.raises(ValueError, match="fit"):
+        eng.forward_paged(_tokens(60, 4), [60, 0], cache)
+    assert int(cache.status) == 4
+    # a request that outgrows its table row
+    small = eng.new_paged_cache(1, n_pages=20, page_size=page, max_len=32)
+    eng.forward_paged(_tokens(32, 5), [32], small)
+    with pytest.raises(ValueError, match="fit"):
+        eng.forward_paged(_tokens(1, 6), [1], small)
+    assert small.lens.tolist() == [32]
