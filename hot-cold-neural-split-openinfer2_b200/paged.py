@@ -403,7 +403,11 @@ class PagedKVCache:
         return self.k[layer], self.v[layer], self.k_scale[layer], self.v_scale[layer]
 
     def plan(self, q_lens: torch.Tensor, n_rows: int) -> PagePlan:
-        """Places ``q_lens[r]`` new tokens of every request (device int32 [max_requests])."""
+        """Places ``q_lens[r]`` new tokens of every request (device int32 [max_requests]).
+        A step that takes a request past ``max_len`` does not work out, whatever its last page has room for."""
+        if self.max_len % self.page_size:          # else the table's width says it
+            _vector(q_lens, "q_lens", _I32, self.max_requests, self.lens.get_device())
+            q_lens = q_lens.masked_fill(q_lens > self.max_len - self.lens, -1)
         return page_plan(self.lens, q_lens, self.tables, self.free_pages, self.n_free, self.page_size, n_rows,
                          self.status)
 

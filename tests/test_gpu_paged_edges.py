@@ -120,3 +120,26 @@ def test_keys_that_are_not_finite(P, N, rows, dim, rotary, interleaved, dtype):
     P.rope_append(q, k, v, cos, sin, pos, pos, *cache, interleaved=interleaved, status=st)
     assert int(st) == N.HC_ERR_RANGE
     _check_append(cache, before, want.cuda(), v, pos)
+
+
+# ─── the cache object ─────────────────────────────────────────────────────────
+@pytest.mark.parametrize("max_len,page", [(20, 16), (1, 16), (127, 64), (64, 64)])
+def test_paged_cache_holds_max_len_positions(P, N, max_len, page):
+    """Not as many as its last page has room for: tables of angles end there."""
+    c = P.PagedKVCache(1, 1, 64, 8, page_size=page, max_requests=2, max_len=max_len)
+    plan = c.plan(_i32([max_len, 0]), max_len)
+    assert plan.positions.tolist() == list(range(max_len)) and plan.kv_lens.tolist() == [max_len, 0]
+    c.commit(plan)
+    c.check()
+    free = int(c.n_free)
+    for q_lens in ([1, 0], [0, max_len + 1], [2 ** 31 - 1, 0]):
+        plan = c.plan(_i32(q_lens), max_len + 1)
+        assert (plan.slots == -1).all() and int(c.n_free) == free and plan.kv_lens.tolist() == [max_len, 0]
+        with pytest.raises(N.HotColdError):
+            c.check()
+        c.status.zero_()
+    plan = c.plan(_i32([0, max_len]), max_len + 1)                    # the other request has its room still
+    assert plan.kv_lens.tolist() == [max_len, max_len]
+    c.check()
+    with pytest.raises(ValueError):
+        c.plan(_i32([1]), 1)

@@ -47,3 +47,17 @@ def test_forward_paged_refuses_a_step_without_pages(make):
     with pytest.raises(ValueError, match="fit"):
         eng.forward_paged(_tokens(1, 6), [1], small)
     assert small.lens.tolist() == [32]
+
+
+def test_forward_paged_refuses_positions_past_max_len(make):
+    """max_len is not a multiple of the page: the rest of the last page is not for use."""
+    eng = make()
+    cache = eng.new_paged_cache(2, page_size=16, max_len=20)
+    eng.forward_paged(_tokens(19, 1), [19], cache)
+    with pytest.raises(ValueError, match="20 positions"):
+        eng.forward_paged(_tokens(2, 2), [2], cache)
+    eng.forward_paged(_tokens(1, 3), [1], cache)
+    with pytest.raises(ValueError, match="20 positions"):
+        eng.forward_paged(_tokens(1, 4), [1], cache)
+    assert cache.lens.tolist() == [20, 0]
+    cache.check()
