@@ -219,50 +219,76 @@ struct ReleaseArgs {
 };
 
 // The pages of the finished requests go back onto the stack, request order
-// then page order.  One CTA, bound by latency like the plan: a serving step
+// then page order.  Their rows are read whole, by as many warps each as there
+// are for so few rows: a search for the end of the prefix would miss a page
+// behind a hole.  One CTA, bound by latency like the plan: a serving step
 // releases a few requests.
 __global__ void __launch_bounds__(PLAN_THREADS) page_release_kernel(const ReleaseArgs p) {
-  __shared__ int32_t s_put[MAX_REQ + 1];
+  __shared__ int32_t s_put[MAX_REQ], s_end[MAX_REQ], s_done[MAX_REQ];
   __shared__ int64_t wsum[32][2];
   __shared__ int s_bad;
-  const int t = threadIdx.x;
+  constexpr int WARPS = PLAN_THREADS / 32;
+  const int t = threadIdx.x, lane = t & 31, w = t >> 5;
   const int per = (p.n_req + PLAN_THREADS - 1) / PLAN_THREADS;
   const int n_free = *p.n_free;
   if (t == 0) s_bad = n_free < 0 || n_free > p.n_pages;
-  __syncthreads();
-  int64_t put = 0, unused = 0;
+  // the finished requests, in order
+  int64_t mine = 0, unused = 0;
   for (int i = 0; i < per; ++i) {
     const int r = t * per + i;
     if (r >= p.n_req) break;
-    const int n = p.done[r] ? first_missing(p.tables + r * p.stride, 0, p.width) : 0;
-    s_put[r] = n;
-    put += n;
+    s_put[r] = s_end[r] = 0;
+    mine += p.done[r] != 0;
+  }
+  int64_t upto = mine;
+  block_scan2(upto, unused, wsum);
+  const int n_done = (int)wsum[31][0];
+  for (int i = 0, at = (int)(upto - mine); i < per; ++i) {
+    const int r = t * per + i;
+    if (r < p.n_req && p.done[r]) s_done[at++] = r;
+  }
+  __syncthreads();
+  // filled entries of their rows, and where the last one ends
+  int share = WARPS;                  // warps of a row
+  while (share > 1 && share * n_done > WARPS) share /= 2;
+  for (int i = w / share; i < n_done; i += WARPS / share) {
+    const int r = s_done[i];
+    const int32_t* row = p.tables + r * p.stride;
+#pragma unroll 4
+    for (unsigned at = w % share * 32; at < (unsigned)p.width; at += share * 32) {
+      const int32_t page = at + lane < (unsigned)p.width ? row[at + lane] : -1;
+      const uint32_t filled = __ballot_sync(0xffffffffu, page >= 0);
+      if (page >= p.n_pages) s_bad = 1;
+      if (lane == 0 && filled) {
+        atomicAdd(&s_put[r], __popc(filled));
+        atomicMax(&s_end[r], (int)(at + 32 - __clz(filled)));
+      }
+    }
+  }
+  __syncthreads();
+  int64_t put = 0;
+  for (int i = 0; i < per; ++i) {
+    const int r = t * per + i;
+    if (r >= p.n_req) break;
+    if (s_put[r] != s_end[r]) s_bad = 1;                 // a hole
+    put += s_put[r];
   }
   int64_t in = put;
   block_scan2(in, unused, wsum);
   const int64_t total = wsum[31][0];
+  if (s_bad || n_free + total > p.n_pages) {             // or more pages than there are: nothing is released
+    if (t == 0 && p.status) atomicOr(p.status, HC_ERR_RANGE);
+    return;
+  }
   int64_t a = in - put;
   for (int i = 0; i < per; ++i) {
     const int r = t * per + i;
     if (r >= p.n_req) break;
     const int n = s_put[r];
-    s_put[r] = (int32_t)min(a, (int64_t)INT32_MAX);
+    s_put[r] = (int32_t)a;
     a += n;
   }
-  const bool over = n_free + total > p.n_pages;
-  if (t == 0) s_put[p.n_req] = over ? 0 : (int32_t)total;
   __syncthreads();
-  if (!over)
-    for (int m = t; m < (int)total; m += PLAN_THREADS) {
-      const int r = owner(s_put, p.n_req, m);
-      const int32_t page = p.tables[r * p.stride + m - s_put[r]];
-      if (page < 0 || page >= p.n_pages) s_bad = 1;      // a hole in a row, too
-    }
-  __syncthreads();
-  if (over || s_bad) {                // more pages than there are: nothing is released
-    if (t == 0 && p.status) atomicOr(p.status, HC_ERR_RANGE);
-    return;
-  }
   for (int m = t; m < (int)total; m += PLAN_THREADS) {
     const int r = owner(s_put, p.n_req, m);
     int32_t* at = p.tables + r * p.stride + m - s_put[r];

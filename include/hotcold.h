@@ -589,8 +589,8 @@ HC_API int hc_page_plan(const int32_t* starts, const int32_t* q_lens, int32_t n_
 /*
  * hc_page_release -- the pages of every request with done[r] != 0 go back
  * onto the stack and its table row becomes missing (-1).  More pages than
- * n_pages in all, or an id outside [0, n_pages): HC_ERR_RANGE and nothing is
- * released.  A page shared by two tables is not known here: release one.
+ * n_pages in all, an id not below n_pages, or a page behind a missing one:
+ * HC_ERR_RANGE and nothing is released.  A page shared by two tables is not known here: release one.
  */
 HC_API int hc_page_release(const uint8_t* done, int32_t n_requests, int32_t* tables, int64_t table_stride,
                            int32_t table_width, int32_t* free_pages, int32_t n_pages, int32_t* n_free,

@@ -143,3 +143,47 @@ def test_paged_cache_holds_max_len_positions(P, N, max_len, page):
     c.check()
     with pytest.raises(ValueError):
         c.plan(_i32([1]), 1)
+
+
+# ─── page release ─────────────────────────────────────────────────────────────
+@pytest.mark.parametrize("row", [
+    [3, -1, -1, 7, -1], [3, -1, 5, -1, -1, -1], [1, 2, 3, 4, -1, 5, 6, -1], [-1, -1, -1, -1, 8],
+    [-1, 3, -1, -1, -1, -1, -1, -1, -1], list(range(1, 34)) + [-1] * 40 + [40] + [-1] * 30,
+])
+def test_page_release_of_a_row_with_any_hole(P, N, row):
+    tables = _i32([row, [0] + [-1] * (len(row) - 1)])
+    free, n_free, st = _i32([9] + [-1] * 99), _i32([1]), N.new_status("cuda")
+    before = tables.clone()
+    P.page_release(torch.tensor([True, True], device="cuda"), tables, free, n_free, st)
+    assert int(st) == N.HC_ERR_RANGE and int(n_free) == 1 and torch.equal(tables, before)
+    assert free.tolist() == [9] + [-1] * 99
+    # a request that goes on may hold what it likes
+    st.zero_()
+    P.page_release(torch.tensor([False, True], device="cuda"), tables, free, n_free, st)
+    N.read_status(st, "page_release")
+    assert int(n_free) == 2 and free[:2].tolist() == [9, 0] and torch.equal(tables[0], before[0])
+
+
+@pytest.mark.parametrize("requests,width,every", [(2048, 70, 1), (2047, 33, 3), (1025, 5, 2), (40, 300, 1), (3, 9000, 1),
+                                                  (1, 1, 1), (33, 64, 5)])
+def test_page_release_of_many_requests_and_wide_tables(P, N, requests, width, every):
+    rng = np.random.default_rng(requests)
+    held = rng.integers(0, width + 1, requests)
+    held[0] = width
+    order = rng.permutation(int(held.sum()) + 7).astype(np.int32)
+    wide = np.full((requests, width + 3), 5, np.int32)                 # what lies past a row's width is not the table's
+    wide[:, :width] = -1
+    at = np.concatenate([[0], np.cumsum(held)])
+    for r in range(requests):
+        wide[r, :held[r]] = order[at[r]:at[r + 1]]
+    free = np.full(len(order), -1, np.int32)
+    free[:7] = order[at[-1]:]
+    done = np.arange(requests) % every == 0
+    dt, dfree, dn, st = torch.tensor(wide).cuda(), torch.tensor(free).cuda(), _i32([7]), N.new_status("cuda")
+    P.page_release(torch.tensor(done).cuda(), dt[:, :width], dfree, dn, st)
+    N.read_status(st, "page_release")
+    back = np.concatenate([wide[r, :held[r]] for r in range(requests) if done[r]])
+    free[7:7 + len(back)] = back
+    wide[done, :width] = -1
+    assert int(dn) == 7 + len(back)
+    assert np.array_equal(dfree.cpu().numpy(), free) and np.array_equal(dt.cpu().numpy(), wide)
