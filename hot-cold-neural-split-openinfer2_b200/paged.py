@@ -418,7 +418,7 @@ class PagedKVCache:
     def release(self, done: torch.Tensor):
         """Frees the pages of the requests with ``done[r]`` (device bool [max_requests])."""
         page_release(done, self.tables, self.free_pages, self.n_free, self.status)
-        self.lens.masked_fill_(done, 0)
+        self.lens.masked_fill_(done & (self.tables[:, 0] < 0), 0)       # a release that was refused leaves the pages
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, plan: PagePlan):
         kv_append(k, v, plan.slots, *self[layer], status=self.status)

@@ -187,3 +187,19 @@ def test_page_release_of_many_requests_and_wide_tables(P, N, requests, width, ev
     wide[done, :width] = -1
     assert int(dn) == 7 + len(back)
     assert np.array_equal(dfree.cpu().numpy(), free) and np.array_equal(dt.cpu().numpy(), wide)
+
+
+def test_paged_cache_release_that_is_refused_keeps_the_lengths(P, N):
+    c = P.PagedKVCache(1, 1, 64, 8, page_size=16, max_requests=3, max_len=64)
+    c.commit(c.plan(_i32([40, 5, 0]), 45))
+    page = int(c.tables[0, 1])
+    c.tables[0, 1] = -1
+    c.release(torch.ones(3, dtype=torch.bool, device="cuda"))
+    with pytest.raises(N.HotColdError):
+        c.check()
+    assert c.lens.tolist() == [40, 5, 0] and int(c.n_free) == 4
+    c.status.zero_()
+    c.tables[0, 1] = page
+    c.release(torch.tensor([True, False, True], device="cuda"))
+    c.check()
+    assert c.lens.tolist() == [0, 5, 0] and int(c.n_free) == 7
