@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import warnings
 from pathlib import Path
 from typing import Optional, Sequence
 
@@ -866,6 +867,23 @@ def build_rope_cache(max_seq_len: int, head_dim: int, theta: float, device=None)
     return torch.cos(ang), torch.sin(ang)
 
 
+def _rope_scaling(cfg: dict) -> Optional[dict]:
+    """The configuration's ``rope_scaling`` as paged.rope_frequencies takes it: a stock entry that leaves the
+    original length out means max_position_embeddings.  One of an unknown kind, or without a number that its kind
+    needs, is left aside with a warning: the model then runs unscaled."""
+    scaling = cfg.get("rope_scaling")
+    if not scaling:
+        return None
+    kind = scaling.get("rope_type") or scaling.get("type") or "default"
+    if kind == "default":
+        return None
+    if any(scaling.get(n) is None for n in paged.ROPE_SCALINGS.get(kind, (kind,))):
+        warnings.warn(f"rope_scaling {scaling} is not known: positions are not scaled")
+        return None
+    original = scaling.get("original_max_position_embeddings") or cfg.get("max_position_embeddings")
+    return {**scaling, "rope_type": kind, "original_max_position_embeddings": original}
+
+
 def _rotate(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
     """Rotary embedding of x [B, heads, T, D] (halves rotated as pairs,
     engine.py:143-158); cos / sin [T, D/2] are cast to x's dtype first."""
@@ -922,7 +940,7 @@ class GroupedQueryAttention(nn.Module):
             self.qkv_w8 = torch.cat([w8("q_proj"), w8("k_proj"), w8("v_proj")], dim=0).contiguous()
             self.o_w8 = w8("o_proj").contiguous()
         # rotary layout of the configuration: part of the head, neighbouring pairs
-        self.rotary_dim = int(self.head_dim * cfg.get("partial_rotary_factor", 1.0))
+        self.rotary_dim = int(self.head_dim * (cfg.get("partial_rotary_factor") or 1.0))
         self.rope_interleaved = bool(cfg.get("rope_interleaved", False))
         self.plain_rope = self.rotary_dim == self.head_dim and not self.rope_interleaved
         self.norm = nn.RMSNorm(self.hidden, eps=cfg["rms_norm_eps"]).to(dev)
@@ -1125,7 +1143,7 @@ class DesdemonaEngine(nn.Module):
             for li in range(self.num_layers)])
         del shared
         self.requires_grad_(False)
-        rotary, scaling = self.attention_layers[0].rotary_dim, cfg.get("rope_scaling")
+        rotary, scaling = self.attention_layers[0].rotary_dim, _rope_scaling(cfg)
         if scaling or rotary != self.head_dim:
             self.cos_cache, self.sin_cache = paged.rope_tables(self.max_seq, rotary, cfg["rope_theta"], scaling, dev)
         else:

@@ -35,6 +35,9 @@ import hc_native as N
 _DTYPES = {torch.float16: N.HC_F16, torch.bfloat16: N.HC_BF16}
 PAGE_SIZES = (16, 32, 64, 128)
 MAX_REQUESTS = 2048             # of one call
+# scalings of rope_frequencies and the numbers that each cannot do without, beside the original length
+ROPE_SCALINGS = {"linear": ("factor",), "dynamic": ("factor",), "yarn": ("factor",),
+                 "llama3": ("factor", "low_freq_factor", "high_freq_factor")}
 
 
 # ─── Argument checks ──────────────────────────────────────────────────────────

@@ -61,3 +61,14 @@ def test_forward_paged_refuses_positions_past_max_len(make):
         eng.forward_paged(_tokens(1, 4), [1], cache)
     assert cache.lens.tolist() == [20, 0]
     cache.check()
+
+
+def test_engine_builds_with_stock_rope_scaling(make):
+    plain = make().cos_cache
+    for stock, same in (({"type": "yarn", "factor": 4.0}, False), ({"type": "dynamic", "factor": 2.0}, True),
+                        ({"rope_type": "default"}, True)):       # dynamic: the engine ends at the original length
+        got = make(rope_scaling=stock).cos_cache
+        assert ((got - plain).abs().max() < 1e-3) == same          # fp32 angles against 64-bit ones
+    with pytest.warns(UserWarning, match="not scaled"):
+        eng = make(rope_scaling={"type": "longrope", "factor": 4.0}, partial_rotary_factor=None)
+    assert torch.equal(eng.cos_cache, plain)

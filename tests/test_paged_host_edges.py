@@ -1,0 +1,35 @@
+"""Host side of the paged serving path at the edges of what it takes (no GPU)."""
+import warnings
+
+import pytest
+
+
+def test_stock_rope_scaling_entries():
+    """What model configurations hold builds an engine: an original length that is left out is the configuration's
+    own, a kind that is not known is left aside and said so."""
+    import engine
+    import paged
+    base = {"max_position_embeddings": 4096, "rope_theta": 10000.0}
+
+    def read(scaling):
+        return engine._rope_scaling({**base, "rope_scaling": scaling})
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        for none in (None, {}, {"rope_type": "default"}, {"type": "default", "factor": 2.0}, {"rope_type": None}):
+            assert read(none) is None
+        assert engine._rope_scaling(base) is None
+        for stock in ({"type": "dynamic", "factor": 2.0}, {"type": "yarn", "factor": 4.0},
+                      {"rope_type": "linear", "type": "linear", "factor": 2.0},
+                      {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0}):
+            got = read(stock)
+            assert got["original_max_position_embeddings"] == 4096
+            freq, _ = paged.rope_frequencies(128, 10000.0, got, 8192)
+            apart, _ = paged.rope_frequencies(128, 10000.0, {**stock, "original_max_position_embeddings": 4096}, 8192)
+            plain, _ = paged.rope_frequencies(128, 10000.0)
+            assert (freq == apart).all() and not (freq == plain).all()
+        given = read({"type": "yarn", "factor": 4.0, "original_max_position_embeddings": 1024})
+        assert given["original_max_position_embeddings"] == 1024
+    for odd in ({"type": "longrope", "long_factor": [1.0], "short_factor": [1.0]}, {"rope_type": "yarn"},
+                {"type": "linear", "factor": None}, {"rope_type": "llama3", "factor": 8.0}):
+        with pytest.warns(UserWarning, match="not scaled"):
+            assert read(odd) is None
