@@ -370,6 +370,23 @@ def _load_base_model(base_model, trust_remote_code: bool):
                                                 trust_remote_code=trust_remote_code)
 
 
+def _rotary_config(hf) -> dict:
+    """The rotary part of a model's configuration, for split_config.json: rope_theta, as the reference writes it
+    (splitter.py:265-292), and what the engine reads beside it, only where the model has it: a scaling, a part of the
+    head, neighbouring pairs.  Configurations that keep theta among the rope parameters are read there."""
+    rope = getattr(hf, "rope_scaling", None) or getattr(hf, "rope_parameters", None)
+    rope = dict(rope) if isinstance(rope, dict) else {}
+    config = {"rope_theta": getattr(hf, "rope_theta", rope.get("rope_theta", 10000.0))}
+    if (rope.get("rope_type") or rope.get("type") or "default") != "default":
+        config["rope_scaling"] = rope
+    part = getattr(hf, "partial_rotary_factor", None) or rope.get("partial_rotary_factor")
+    if part is not None and part != 1.0:
+        config["partial_rotary_factor"] = part
+    if getattr(hf, "rope_interleaved", False):
+        config["rope_interleaved"] = True
+    return config
+
+
 def split_dense(base_model, profile_path: str, output_dir: str, hot_count: int = HOT_COUNT_DENSE,
                 trust_remote_code: bool = False, device="cuda") -> dict:
     """The reference's split-dense step (splitter.py:129-302) on the GPU.
@@ -471,7 +488,7 @@ def split_dense(base_model, profile_path: str, output_dir: str, hot_count: int =
         "vocab_size": hf.vocab_size,
         "num_attention_heads": hf.num_attention_heads,
         "num_key_value_heads": hf.num_key_value_heads,
-        "rope_theta": getattr(hf, "rope_theta", 10000.0),
+        **_rotary_config(hf),
         "rms_norm_eps": hf.rms_norm_eps,
         "hidden_act": hf.hidden_act,
         "act_on_both": getattr(hf, "model_type", "") == "bamboo",

@@ -72,3 +72,28 @@ def test_engine_builds_with_stock_rope_scaling(make):
     with pytest.warns(UserWarning, match="not scaled"):
         eng = make(rope_scaling={"type": "longrope", "factor": 4.0}, partial_rotary_factor=None)
     assert torch.equal(eng.cos_cache, plain)
+
+
+def test_split_to_engine_keeps_the_rotary_layout(tmp_path):
+    """From a model's configuration through split_dense to the engine's tables."""
+    import json
+    import os
+    import sys
+
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    sys.path.insert(0, os.path.join(os.path.dirname(__file__), "golden"))
+    import engine
+    import paged
+    import splitter
+    import stub_models
+    model = stub_models.engine_stub_model()
+    model.config.rope_scaling = {"rope_type": "linear", "factor": 4.0}
+    model.config.partial_rotary_factor = 0.5
+    profile = tmp_path / "profile.json"
+    profile.write_text(json.dumps(stub_models.engine_stub_profile()))
+    splitter.split_dense(model, str(profile), str(tmp_path / "split"), hot_count=16)
+    eng = engine.DesdemonaEngine(str(tmp_path / "split"), max_seq_len=64)
+    cos, sin = paged.rope_tables(64, 64, 10000.0, {"rope_type": "linear", "factor": 4.0}, device="cuda")
+    assert torch.equal(eng.cos_cache, cos) and torch.equal(eng.sin_cache, sin)
+    assert len(eng.generate_batch([_tokens(5, 1) % 64, _tokens(9, 2) % 64], 4, temperature=0.0)[1]) == 4

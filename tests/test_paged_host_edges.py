@@ -33,3 +33,25 @@ def test_stock_rope_scaling_entries():
                 {"type": "linear", "factor": None}, {"rope_type": "llama3", "factor": 8.0}):
         with pytest.warns(UserWarning, match="not scaled"):
             assert read(odd) is None
+
+
+def test_split_config_carries_the_rotary_layout():
+    """A model's scaling, partial head and pair layout reach the engine; a plain one is written as before."""
+    from types import SimpleNamespace as C
+
+    import engine
+    import splitter
+    llama = {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0,
+             "original_max_position_embeddings": 8192}
+    for plain in (C(rope_theta=500000.0), C(rope_theta=500000.0, rope_scaling=None),
+                  C(rope_parameters={"rope_theta": 500000.0, "rope_type": "default"}),
+                  C(rope_theta=500000.0, partial_rotary_factor=1.0, rope_interleaved=False)):
+        assert splitter._rotary_config(plain) == {"rope_theta": 500000.0}
+    assert splitter._rotary_config(C()) == {"rope_theta": 10000.0}
+    got = splitter._rotary_config(C(rope_theta=500000.0, rope_scaling=llama))
+    assert got == {"rope_theta": 500000.0, "rope_scaling": llama}
+    got = splitter._rotary_config(C(rope_parameters={**llama, "rope_theta": 500000.0, "partial_rotary_factor": 0.5}))
+    assert got["rope_theta"] == 500000.0 and got["partial_rotary_factor"] == 0.5
+    assert engine._rope_scaling({**got, "max_position_embeddings": 131072})["factor"] == 8.0
+    got = splitter._rotary_config(C(rope_theta=1e4, partial_rotary_factor=0.25, rope_interleaved=True))
+    assert got == {"rope_theta": 1e4, "partial_rotary_factor": 0.25, "rope_interleaved": True}
