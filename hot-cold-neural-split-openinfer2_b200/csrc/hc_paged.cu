@@ -17,6 +17,7 @@ using namespace hc;
 namespace cg = cooperative_groups;
 
 constexpr int MAX_REQ = 2048;           // requests of one step (their offsets sit in shared memory)
+constexpr int MAX_ROWS = 1 << 30;       // rows of one call: 32-bit row indices step past the last one by a grid's width
 constexpr int PLAN_THREADS = 1024;
 constexpr int PLAN_CL = 8;              // CTAs of a plan with many rows (one cluster)
 
@@ -827,7 +828,7 @@ int check_rope(const hc_rope_args* a, bool to_cache) {
   if (!aligned(a->q, 2) || !aligned(a->k, 2) || !aligned(a->q_out, 2) || !aligned(a->k_out, 2) ||
       !aligned(a->cos_t, 4) || !aligned(a->sin_t, 4) || !aligned(a->positions, 8))
     return HC_ERR_ARG;
-  return HC_OK;
+  return a->n_rows > MAX_ROWS ? HC_ERR_UNSUPPORTED : HC_OK;
 }
 
 // The vector form wants 16-byte pieces throughout and whole units of 8 pairs.
@@ -1016,7 +1017,7 @@ extern "C" int hc_page_plan(const int32_t* starts, const int32_t* q_lens, int32_
   if (n_requests <= 0 || table_width <= 0 || table_stride < table_width || n_pages <= 0 || page_size <= 0)
     return HC_ERR_ARG;
   if ((int64_t)table_width * page_size > INT32_MAX) return HC_ERR_ARG;
-  if (n_requests > MAX_REQ) return HC_ERR_UNSUPPORTED;
+  if (n_requests > MAX_REQ || n_rows > MAX_ROWS) return HC_ERR_UNSUPPORTED;
   PlanArgs p = {starts, q_lens, n_requests, tables, table_stride, table_width, free_pages, n_pages, n_free,
                 page_size, n_rows, cu_q, kv_lens, positions, slots, status};
   const int cl = n_rows > PLAN_THREADS ? PLAN_CL : 1;
@@ -1068,6 +1069,7 @@ extern "C" int hc_kv_append(const hc_kv_pages* cache, const void* k, int64_t k_r
                             int32_t* status, hc_stream_t stream) {
   if (n_rows < 0 || (n_rows && (!k || !v || !slots)) || (dtype != HC_F16 && dtype != HC_BF16)) return HC_ERR_ARG;
   if (!aligned(k, 2) || !aligned(v, 2) || !aligned(slots, 8)) return HC_ERR_ARG;
+  if (n_rows > MAX_ROWS) return HC_ERR_UNSUPPORTED;
   const int rc = check_pages(cache);
   if (rc != HC_OK) return rc;
   if (n_rows == 0) return HC_OK;

@@ -545,7 +545,8 @@ HC_API int hc_attn_decode(const void* qkv, const float* cos_t, const float* sin_
  * they were.  A request's token at position pos lies at slot
  * tables[r][pos / page_size] * page_size + pos % page_size of the cache.
  * The order of a layer is hc_page_plan (once per step), hc_rope_append,
- * hc_paged_attn.  `status` may be NULL in all of them.
+ * hc_paged_attn.  `status` may be NULL in all of them.  A call takes up to
+ * 2^30 rows (else HC_ERR_UNSUPPORTED).
  */
 
 /*

@@ -55,3 +55,20 @@ def test_split_config_carries_the_rotary_layout():
     assert engine._rope_scaling({**got, "max_position_embeddings": 131072})["factor"] == 8.0
     got = splitter._rotary_config(C(rope_theta=1e4, partial_rotary_factor=0.25, rope_interleaved=True))
     assert got == {"rope_theta": 1e4, "partial_rotary_factor": 0.25, "rope_interleaved": True}
+
+
+def test_row_counts_past_the_index_range_are_refused():
+    """Row indices are 32-bit and step past the last row by a grid's width."""
+    import ctypes
+
+    import hc_native as N
+    from test_paged_host import FAKE, _pages, _rope
+    for rows, pages in (((1 << 30) + 1, {}), ((1 << 31) - 1, {}), ((1 << 31) - 32, {"head_dim": 64})):
+        assert N.lib.hc_page_plan(FAKE, FAKE, 1, FAKE, 8, 8, FAKE, 4, FAKE, 16, rows, FAKE, FAKE, FAKE, FAKE, None,
+                                  None) == N.HC_ERR_UNSUPPORTED
+        c = ctypes.byref(_pages(N, **pages))
+        a = _rope(N, n_rows=rows, head_dim=pages.get("head_dim", 128), rotary_dim=64)
+        assert N.lib.hc_rope(ctypes.byref(a), None, None) == N.HC_ERR_UNSUPPORTED
+        assert N.lib.hc_kv_append(c, FAKE, 0, 128, FAKE, 0, 128, FAKE, rows, N.HC_F16, None,
+                                  None) == N.HC_ERR_UNSUPPORTED
+        assert N.lib.hc_rope_append(ctypes.byref(a), c, FAKE, 0, 128, FAKE, None, None) == N.HC_ERR_UNSUPPORTED
