@@ -816,6 +816,8 @@ __global__ void __launch_bounds__(APPEND_THREADS, ROWS == FEW ? 4 : 2)
 // ---------------------------------------------------------------------------
 inline bool multiple(int64_t v, int64_t m) { return v % m == 0; }
 inline bool aligned(const void* ptr, uintptr_t a) { return (reinterpret_cast<uintptr_t>(ptr) & (a - 1)) == 0; }
+template <typename... P>
+inline bool all_aligned(uintptr_t a, const P*... ptr) { return (aligned(ptr, a) && ...); }
 
 int check_rope(const hc_rope_args* a, bool to_cache) {
   if (!a || !a->cos_t || !a->sin_t) return HC_ERR_ARG;
@@ -1014,6 +1016,9 @@ extern "C" int hc_page_plan(const int32_t* starts, const int32_t* q_lens, int32_
                             int64_t* positions, int64_t* slots, int32_t* status, hc_stream_t stream) {
   if (!starts || !q_lens || !tables || !free_pages || !n_free || !cu_q || !kv_lens) return HC_ERR_ARG;
   if (n_rows < 0 || (n_rows && (!positions || !slots))) return HC_ERR_ARG;
+  if (!all_aligned(4, starts, q_lens, tables, free_pages, n_free, cu_q, kv_lens, status) ||
+      !all_aligned(8, positions, slots))
+    return HC_ERR_ARG;
   if (n_requests <= 0 || table_width <= 0 || table_stride < table_width || n_pages <= 0 || page_size <= 0)
     return HC_ERR_ARG;
   if ((int64_t)table_width * page_size > INT32_MAX) return HC_ERR_ARG;
@@ -1038,7 +1043,8 @@ extern "C" int hc_page_plan(const int32_t* starts, const int32_t* q_lens, int32_
 extern "C" int hc_page_release(const uint8_t* done, int32_t n_requests, int32_t* tables, int64_t table_stride,
                                int32_t table_width, int32_t* free_pages, int32_t n_pages, int32_t* n_free,
                                int32_t* status, hc_stream_t stream) {
-  if (!done || !tables || !free_pages || !n_free) return HC_ERR_ARG;
+  if (!done || !tables || !free_pages || !n_free || !all_aligned(4, tables, free_pages, n_free, status))
+    return HC_ERR_ARG;
   if (n_requests <= 0 || table_width <= 0 || table_stride < table_width || n_pages <= 0) return HC_ERR_ARG;
   if (n_requests > MAX_REQ) return HC_ERR_UNSUPPORTED;
   ReleaseArgs p = {done, n_requests, tables, table_stride, table_width, free_pages, n_pages, n_free, status};
@@ -1049,6 +1055,7 @@ extern "C" int hc_page_release(const uint8_t* done, int32_t n_requests, int32_t*
 extern "C" int hc_rope(const hc_rope_args* a, int32_t* status, hc_stream_t stream) {
   const int rc = check_rope(a, false);
   if (rc != HC_OK) return rc;
+  if (!aligned(status, 4)) return HC_ERR_ARG;
   if (a->n_rows == 0) return HC_OK;
   const bool vec = rope_vec(a, true);
   RopeArgs p = rope_args(a, true, status);
@@ -1068,7 +1075,7 @@ extern "C" int hc_kv_append(const hc_kv_pages* cache, const void* k, int64_t k_r
                             int64_t v_row, int64_t v_head, const int64_t* slots, int32_t n_rows, int32_t dtype,
                             int32_t* status, hc_stream_t stream) {
   if (n_rows < 0 || (n_rows && (!k || !v || !slots)) || (dtype != HC_F16 && dtype != HC_BF16)) return HC_ERR_ARG;
-  if (!aligned(k, 2) || !aligned(v, 2) || !aligned(slots, 8)) return HC_ERR_ARG;
+  if (!all_aligned(2, k, v) || !aligned(slots, 8) || !aligned(status, 4)) return HC_ERR_ARG;
   if (n_rows > MAX_ROWS) return HC_ERR_UNSUPPORTED;
   const int rc = check_pages(cache);
   if (rc != HC_OK) return rc;
@@ -1082,7 +1089,7 @@ extern "C" int hc_rope_append(const hc_rope_args* a, const hc_kv_pages* cache, c
                               int64_t v_head, const int64_t* slots, int32_t* status, hc_stream_t stream) {
   int rc = check_rope(a, true);
   if (rc != HC_OK) return rc;
-  if ((a->n_rows && (!v || !slots)) || !aligned(v, 2) || !aligned(slots, 8)) return HC_ERR_ARG;
+  if ((a->n_rows && (!v || !slots)) || !aligned(v, 2) || !aligned(slots, 8) || !aligned(status, 4)) return HC_ERR_ARG;
   rc = check_pages(cache);
   if (rc != HC_OK) return rc;
   if (a->n_kv_heads != cache->n_kv_heads || a->head_dim != cache->head_dim) return HC_ERR_ARG;

@@ -641,7 +641,8 @@ extern "C" int hc_paged_attn(const hc_attn_args* a, const hc_kv_pages* c, void* 
     return HC_ERR_ARG;
   if (a->q_row < 0 || a->q_head < 0 || a->out_row < 0 || a->out_head < 0) return HC_ERR_ARG;
   if (!aligned(a->q, 2) || !aligned(a->out, 2) || !aligned(a->lse, 4) || !aligned(c->k, 16) || !aligned(c->v, 16) ||
-      !aligned(a->tables, 4) || !aligned(c->k_scale, 4) || !aligned(c->v_scale, 4))
+      !aligned(a->tables, 4) || !aligned(c->k_scale, 4) || !aligned(c->v_scale, 4) || !aligned(a->cu_q, 4) ||
+      !aligned(a->kv_lens, 4) || !aligned(status, 4))
     return HC_ERR_ARG;
   if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128)
     return HC_ERR_UNSUPPORTED;

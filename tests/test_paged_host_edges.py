@@ -72,3 +72,28 @@ def test_row_counts_past_the_index_range_are_refused():
         assert N.lib.hc_kv_append(c, FAKE, 0, 128, FAKE, 0, 128, FAKE, rows, N.HC_F16, None,
                                   None) == N.HC_ERR_UNSUPPORTED
         assert N.lib.hc_rope_append(ctypes.byref(a), c, FAKE, 0, 128, FAKE, None, None) == N.HC_ERR_UNSUPPORTED
+
+
+def test_misaligned_addresses_are_refused():
+    """Every pointer that a kernel reads or writes through, by the size of what it points to."""
+    import ctypes
+
+    import hc_native as N
+    from test_paged_host import FAKE, _attn, _pages, _rope
+    plan = dict(starts=4, q=4, tables=4, free=4, n_free=4, cu=4, kv=4, pos=8, slots=8, status=4)
+    for name, size in plan.items():
+        p = {n: FAKE + (size // 2 if n == name else 0) for n in plan}
+        assert N.lib.hc_page_plan(p["starts"], p["q"], 1, p["tables"], 8, 8, p["free"], 4, p["n_free"], 16, 4, p["cu"],
+                                  p["kv"], p["pos"], p["slots"], p["status"], None) == N.HC_ERR_ARG, name
+    for bad in ({"tables"}, {"free"}, {"n_free"}, {"status"}):
+        p = {n: FAKE + 2 * (n in bad) for n in ("tables", "free", "n_free", "status")}
+        assert N.lib.hc_page_release(FAKE, 1, p["tables"], 8, 8, p["free"], 4, p["n_free"], p["status"],
+                                     None) == N.HC_ERR_ARG, bad
+    c = ctypes.byref(_pages(N))
+    for kw, status in (({"cu_q": FAKE + 2}, None), ({"kv_lens": FAKE + 1}, None), ({"lse": FAKE + 2}, None),
+                       ({"tables": FAKE + 2}, None), ({}, FAKE + 2)):
+        assert N.lib.hc_paged_attn(ctypes.byref(_attn(N, **kw)), c, FAKE, 1 << 30, status, None) == N.HC_ERR_ARG, kw
+    a = ctypes.byref(_rope(N))
+    assert N.lib.hc_rope(a, FAKE + 2, None) == N.HC_ERR_ARG
+    assert N.lib.hc_kv_append(c, FAKE, 256, 128, FAKE, 256, 128, FAKE, 1, N.HC_F16, FAKE + 1, None) == N.HC_ERR_ARG
+    assert N.lib.hc_rope_append(a, c, FAKE, 256, 128, FAKE, FAKE + 2, None) == N.HC_ERR_ARG
