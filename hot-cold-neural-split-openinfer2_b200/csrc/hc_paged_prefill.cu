@@ -260,7 +260,9 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
   const int t = threadIdx.x, lane = t & 31, w = __shfl_sync(0xffffffffu, t >> 5, 0);
   const uint32_t smem = (smem_u32(raw) + 1023) & ~1023u;
 
-  // The step's work in halves sets the piece length; with it, the pieces of each request.
+  // The step's work in halves sets the piece length; with it, the pieces of each request.  Offsets that go back
+  // anywhere may let the requests (each in range by itself) claim more rows than there are: the grid, the slots and
+  // the 32-bit sums below, which hold for n_rows rows, would not do, and none of these requests is served.
   auto tiles_of = [&](const Req& x) { return (x.q_len * p.g + ROWS - 1) / ROWS; };
   auto halves_of = [](int kv) { return (kv + HALF - 1) / HALF; };
   auto piece_of = [&](int64_t halves) {                 // even
@@ -283,12 +285,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
     if (w == 0) {
       Req x = {0, 0, 0};
       if (lane < p.n_req) s_req[lane] = x = request(p, lane, blockIdx.x == 0);
+      const bool back = __any_sync(0xffffffffu, lane < p.n_req && p.cu_q[lane + 1] < p.cu_q[lane]);
       int64_t sum = (int64_t)tiles_of(x) * p.nkv * halves_of(x.kv);
 #pragma unroll
       for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       const int piece = piece_of(sum);
       const int64_t upto = scan(lane < p.n_req ? units_of(x, piece) : 0);
-      s_pre[lane + 1] = make_int2((int)(upto >> 32), (int)upto);
+      s_pre[lane + 1] = make_int2(back ? -1 : (int)(upto >> 32), (int)upto);
       if (lane == 0) s_pre[0] = make_int2(0, 0), s_piece = piece;
     }
     __syncthreads();
@@ -300,15 +303,17 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
     };
     const int count = max(0, min(per, p.n_req - t * per));
     int64_t sum = 0;
+    bool back = false;
     for (int i = 0; i < count; ++i) {
       const Req x = request(p, t * per + i, blockIdx.x == 0);
       if (p.n_req <= KEPT_REQ) s_req[t * per + i] = x;
       sum += (int64_t)tiles_of(x) * p.nkv * halves_of(x.kv);
+      back |= p.cu_q[t * per + i + 1] < p.cu_q[t * per + i];
     }
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) s_wsum[w] = sum;
-    __syncthreads();
+    back = __syncthreads_or(back);
     sum = 0;
     for (int k = 0; k < PF_THREADS / 32; ++k) sum += s_wsum[k];
     __syncthreads();
@@ -323,14 +328,12 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
     for (int k = 0; k < w; ++k) at += s_wsum[k];
     for (int i = 0; i < count; ++i) {
       at += units_of(mine(i), piece);
-      s_pre[t * per + i + 1] = make_int2((int)(at >> 32), (int)at);
+      s_pre[t * per + i + 1] = make_int2(back ? -1 : (int)(at >> 32), (int)at);
     }
     __syncthreads();
   }
   const int piece = s_piece, all = s_pre[p.n_req].x;
-  // Offsets that go back and forth (each request in range by itself) claim more rows than there are: the grid would
-  // leave pieces out and the join would read slots that nothing wrote.  None of them is served then.
-  const bool over = (unsigned)all > gridDim.x;
+  const bool over = (unsigned)all > gridDim.x;          // -1: none is served
   if (blockIdx.x == 0 && t == 0) {
     p.pf_cuts[0] = make_int4(over ? 0 : s_pre[p.n_req].y, 0, 0, 0);
     if (over && p.status) atomicOr(p.status, HC_ERR_RANGE);

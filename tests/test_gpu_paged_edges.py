@@ -203,3 +203,24 @@ def test_paged_cache_release_that_is_refused_keeps_the_lengths(P, N):
     c.release(torch.tensor([True, False, True], device="cuda"))
     c.check()
     assert c.lens.tolist() == [0, 5, 0] and int(c.n_free) == 7
+
+
+# ─── offsets that claim more rows than there are ──────────────────────────────
+@pytest.mark.parametrize("requests", [4, 40, 300])
+def test_paged_prompt_attention_serves_no_more_rows_than_there_are(P, N, requests):
+    """Two requests of 60 of 100 rows each, the offsets going back between them: both tiles fit the launch, and still
+    neither is served; in order, they are."""
+    page, nq, nkv, dim = 64, 8, 2, 64
+    g = _gen(requests)
+    tables, _, _, n_pages = _step([(300, 0)], page, g)
+    cache = _filled(n_pages, nkv, page, dim, g)
+    tables, kv = tables.expand(requests, -1).contiguous(), _i32([300] * requests)
+    q = torch.randn(100, nq, dim, generator=g, device="cuda").half()
+    out, st = torch.full_like(q, 9.0), N.new_status("cuda")
+    P.paged_attention(q, *cache, tables, _i32([0, 60, 0, 60] + [60] * (requests - 3)), kv, max_q=100, out=out, status=st)
+    assert int(st) == N.HC_ERR_RANGE and (out == 9).all()
+    st.zero_()
+    cu = _i32([0, 60, 60, 100] + [100] * (requests - 3))
+    P.paged_attention(q, *cache, tables, cu, kv, max_q=100, out=out, status=st)
+    N.read_status(st, "paged_attention")
+    _check_attention(out, None, q, cache, tables[:3], cu[:4], kv[:3])
