@@ -10,6 +10,8 @@
 // subnormals.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "hc_common.cuh"
 
 namespace hcp {
@@ -496,6 +498,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const RopeArgs p) {
 // the write of a step's keys and values
 // ---------------------------------------------------------------------------
 constexpr int E_MIN = -40, E_MAX = 40;  // exponents of a page scale
+constexpr float TOP_MAX = 448.0f * (1ll << E_MAX);      // the largest value that a page holds
 constexpr int MANY = 16, FEW = 4;       // rows a warp holds at once
 constexpr int SPLIT_ROWS = 1024;        // rows from which the queries get a launch of their own
 constexpr int APPEND_THREADS = 256;
@@ -684,6 +687,7 @@ __device__ __forceinline__ void append_run(const AppendArgs& p, int which, int h
         }
       }
   }
+  if constexpr (!std::is_same<T, __half>::value) odd |= top > TOP_MAX;       // saturates; no f16 value does
   if (__any_sync(0xffffffffu, odd) && lane == 0 && p.status) atomicOr(p.status, HC_ERR_RANGE);
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));

@@ -640,9 +640,9 @@ HC_API int hc_rope(const hc_rope_args* args, int32_t* status, hc_stream_t stream
  * 40, with |x| <= 448 * 2^e for its finite values.  Rows that begin a page
  * (its first slot among them) begin it anew; rows that enter it later raise
  * the scale when they need to, and the rows before them are rounded again
- * (which changes only values among e4m3's subnormals).  Infinities saturate
- * at 448 times the scale, NaN becomes 0, and both set HC_ERR_RANGE: the cache
- * never holds a NaN.
+ * (which changes only values among e4m3's subnormals).  Infinities, and bf16
+ * values past 448 * 2^40, saturate at 448 times the scale, NaN becomes 0, and
+ * all of them set HC_ERR_RANGE: the cache never holds a NaN.
  */
 HC_API int hc_kv_append(const hc_kv_pages* cache, const void* k, int64_t k_row, int64_t k_head, const void* v,
                         int64_t v_row, int64_t v_head, const int64_t* slots, int32_t n_rows, int32_t dtype,

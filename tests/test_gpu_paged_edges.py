@@ -224,3 +224,21 @@ def test_paged_prompt_attention_serves_no_more_rows_than_there_are(P, N, request
     P.paged_attention(q, *cache, tables, cu, kv, max_q=100, out=out, status=st)
     N.read_status(st, "paged_attention")
     _check_attention(out, None, q, cache, tables[:3], cu[:4], kv[:3])
+
+
+@pytest.mark.parametrize("rows", [1, 1100])
+def test_kv_append_flags_values_past_the_largest_scale(P, N, rows):
+    """448 * 2^40 is held; the next bf16 value saturates, and that is reported like an infinity."""
+    top = 448.0 * 2.0 ** 40
+    x = torch.randn(rows, 1, 64, device="cuda", generator=_gen(rows)).bfloat16()
+    x[rows // 2, 0, 5] = top
+    slots = torch.arange(rows, device="cuda")
+    for value, flagged in ((top, 0), (-top, 0), (450.0 * 2.0 ** 40, N.HC_ERR_RANGE), (-3e38, N.HC_ERR_RANGE)):
+        k = x.clone()
+        k[rows // 2, 0, 5] = value
+        cache = _cache(18, 1, 64, 64, seed=1)
+        before, st = _np(*cache), N.new_status("cuda")
+        P.kv_append(x, k, slots, *cache, status=st)
+        assert int(st) == flagged
+        _check_append(cache, before, x, k, slots)
+        assert k[rows // 2, 0, 5].item() == value or value == -3e38
