@@ -97,3 +97,50 @@ def test_split_to_engine_keeps_the_rotary_layout(tmp_path):
     cos, sin = paged.rope_tables(64, 64, 10000.0, {"rope_type": "linear", "factor": 4.0}, device="cuda")
     assert torch.equal(eng.cos_cache, cos) and torch.equal(eng.sin_cache, sin)
     assert len(eng.generate_batch([_tokens(5, 1) % 64, _tokens(9, 2) % 64], 4, temperature=0.0)[1]) == 4
+
+
+def _follows(eng, prompt, made):
+    """Every token that was made has the plain model's largest logit to the engine's tolerance: an element is off by
+    at most the norm's bound, its own logit and the largest one."""
+    ids = torch.cat([prompt, torch.tensor(made, device="cuda")])[:-1]
+    page = 16
+    cache, plain = eng.new_paged_cache(1, page_size=page), _Plain(eng, 512 // page, page)
+    with torch.inference_mode():
+        plan = cache.plan(torch.tensor([len(ids)], dtype=torch.int32, device="cuda"), len(ids))
+        logits = plain.step(ids, plan, cache.tables.cpu().numpy())[len(prompt) - 1:].double()
+    short = logits.max(-1).values - logits.gather(1, torch.tensor(made, device="cuda")[:, None])[:, 0]
+    return bool((short <= 2 * LOGIT_TOL * logits.norm(dim=-1)).all())
+
+
+def test_generate_batch_follows_the_plain_model(make):
+    """Greedy tokens of three prompts against the plain model, and again with an end token that takes one request out
+    in the middle, whose pages the others then grow into."""
+    eng = make()
+    prompts = [_tokens(n, n) for n in (5, 70, 33)]
+    full = eng.generate_batch(prompts, 40, temperature=0.0, page_size=16)
+    assert [len(r) for r in full] == [40] * 3
+    for p, r in zip(prompts, full):
+        assert _follows(eng, p, r)
+    assert not _follows(eng, prompts[0], full[1])            # the check tells requests apart
+    # an end token that one request makes among its first 15 and the others never do
+    picks = [(r, t) for r in range(3) for t in full[r][:15] if all(t not in full[o] for o in range(3) if o != r)]
+    assert picks
+    for r, eos in (picks[0], picks[-1]):
+        cut = eng.generate_batch(prompts, 40, temperature=0.0, eos_token_id=[eos, VOCAB + 1], page_size=16)
+        for i, (p, row) in enumerate(zip(prompts, cut)):
+            assert _follows(eng, p, row)
+            assert (row.index(eos) == len(row) - 1) if eos in row else len(row) == 40
+        assert cut[r][-1] == eos and len(cut[r]) <= 40
+    eng.check()
+
+
+def test_generate_batch_of_one_is_the_step_by_step_loop(make):
+    eng = make()
+    prompt = _tokens(20, 9)
+    cache, tok, want = eng.new_paged_cache(1, page_size=32, max_len=60), prompt, []
+    for _ in range(24):
+        tok = eng.forward_paged(tok, [len(tok)], cache).argmax(-1)
+        want.append(int(tok))
+    got = eng.generate_batch([prompt], 24, temperature=0.0, page_size=32)[0]
+    assert len(got) == 24 and _follows(eng, prompt, got) and _follows(eng, prompt, want)
+    cache.check()
