@@ -1360,10 +1360,10 @@ class DesdemonaEngine(nn.Module):
         prompts = [p.reshape(-1) for p in prompts]
         n_new = max(int(max_new_tokens), 1)
         lens = [p.shape[0] for p in prompts]
-        if not prompts or min(lens) == 0 or max(lens) + n_new > self.max_seq:
+        if not prompts or min(lens) == 0 or max(lens) + n_new - 1 > self.max_seq:     # the last token is not cached
             raise ValueError(f"prompts must be non-empty and fit {self.max_seq} positions with the new tokens")
-        pages = sum(-(-(n + n_new) // page_size) for n in lens)
-        cache = self.new_paged_cache(len(prompts), pages, page_size, max(lens) + n_new)
+        pages = sum(-(-(n + n_new - 1) // page_size) for n in lens)
+        cache = self.new_paged_cache(len(prompts), pages, page_size, max(lens) + n_new - 1)
         out = torch.empty(len(prompts), n_new, dtype=torch.int64, device=self.device)
         ids = [[] for _ in prompts]
         live = list(range(len(prompts)))

@@ -144,3 +144,15 @@ def test_generate_batch_of_one_is_the_step_by_step_loop(make):
     got = eng.generate_batch([prompt], 24, temperature=0.0, page_size=32)[0]
     assert len(got) == 24 and _follows(eng, prompt, got) and _follows(eng, prompt, want)
     cache.check()
+
+
+def test_generate_batch_up_to_the_last_position(make):
+    """As generate(): the last token that is made takes no position."""
+    eng = make()
+    prompt = _tokens(500, 3)
+    one = eng.generate(prompt, 13, temperature=0.0)
+    got = eng.generate_batch([prompt, prompt[:16]], 13, temperature=0.0, page_size=16)
+    assert [len(r) for r in (one, *got)] == [13] * 3
+    with pytest.raises(ValueError):
+        eng.generate_batch([prompt], 14, temperature=0.0)
+    eng.check()
