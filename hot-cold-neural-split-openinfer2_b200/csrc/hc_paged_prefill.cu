@@ -260,9 +260,15 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
   const int t = threadIdx.x, lane = t & 31, w = __shfl_sync(0xffffffffu, t >> 5, 0);
   const uint32_t smem = (smem_u32(raw) + 1023) & ~1023u;
 
-  // The step's work in halves sets the piece length; with it, the pieces of each request.  Offsets that go back
-  // anywhere may let the requests (each in range by itself) claim more rows than there are: the grid, the slots and
-  // the 32-bit sums below, which hold for n_rows rows, would not do, and none of these requests is served.
+  // The step's work in halves sets the piece length; with it, the pieces of each request.  Where offsets go back the
+  // requests (each in range by itself) may claim more rows than there are: the grid, the slots and the 32-bit sums
+  // below, which hold for n_rows rows, would not do, and none of these requests is served.
+  auto too_many = [&]() {
+    int64_t claimed = 0;
+#pragma unroll 1
+    for (int r = 0; r < p.n_req; ++r) claimed += request(p, r, false).q_len;
+    return claimed > p.n_rows;
+  };
   auto tiles_of = [&](const Req& x) { return (x.q_len * p.g + ROWS - 1) / ROWS; };
   auto halves_of = [](int kv) { return (kv + HALF - 1) / HALF; };
   auto piece_of = [&](int64_t halves) {                 // even
@@ -285,7 +291,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
     if (w == 0) {
       Req x = {0, 0, 0};
       if (lane < p.n_req) s_req[lane] = x = request(p, lane, blockIdx.x == 0);
-      const bool back = __any_sync(0xffffffffu, lane < p.n_req && p.cu_q[lane + 1] < p.cu_q[lane]);
+      const bool back = __any_sync(0xffffffffu, lane < p.n_req && p.cu_q[lane + 1] < p.cu_q[lane]) && too_many();
       int64_t sum = (int64_t)tiles_of(x) * p.nkv * halves_of(x.kv);
 #pragma unroll
       for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -313,7 +319,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) paged_prefill_kernel(const Attn
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) s_wsum[w] = sum;
-    back = __syncthreads_or(back);
+    back = __syncthreads_or(back) && too_many();
     sum = 0;
     for (int k = 0; k < PF_THREADS / 32; ++k) sum += s_wsum[k];
     __syncthreads();

@@ -678,9 +678,9 @@ HC_API int hc_rope_append(const hc_rope_args* args, const hc_kv_pages* cache, co
  * Softmax statistics are fp32; a page id outside the cache, a length past the
  * table or rows past n_rows set HC_ERR_RANGE and are left out.  Bytes of
  * positions behind kv_lens are never used, whatever they hold.
- * A request whose offsets go back is left out with HC_ERR_RANGE, too, and with
- * it every request of more than 16 rows a key-value head: together they could
- * claim more rows than n_rows.
+ * A request whose offsets go back is left out with HC_ERR_RANGE, too; when
+ * such offsets make the others of more than 16 rows a key-value head claim more
+ * rows than n_rows, none of those is served.
  * n_requests <= 2048, n_q_heads / n_kv_heads <= 16, n_rows times that ratio <=
  * 2^30 (else HC_ERR_UNSUPPORTED).
  */

@@ -224,6 +224,13 @@ def test_paged_prompt_attention_serves_no_more_rows_than_there_are(P, N, request
     P.paged_attention(q, *cache, tables, cu, kv, max_q=100, out=out, status=st)
     N.read_status(st, "paged_attention")
     _check_attention(out, None, q, cache, tables[:3], cu[:4], kv[:3])
+    # offsets that end in zeros go back, but claim no row twice: the requests before them are served
+    st.zero_()
+    out.fill_(9.0)
+    P.paged_attention(q, *cache, tables, _i32([0, 60, 60, 100] + [0] * (requests - 3)), kv, max_q=100, out=out,
+                      status=st)
+    assert (int(st) == N.HC_ERR_RANGE) == (requests > 3)
+    _check_attention(out, None, q, cache, tables[:3], cu[:4], kv[:3])
 
 
 @pytest.mark.parametrize("rows", [1, 1100])
