@@ -459,7 +459,8 @@ __device__ __forceinline__ void rope_rows_vec(const RopeArgs& p, int block) {
 }
 
 // Any rotary size, stride and alignment: a row a CTA, a thread per pair or
-// passing element.
+// passing element.  Bound by issue slots (74% busy) and 2-byte accesses: 8192
+// rows of 32 + 8 heads with a rotary size of 90 take 105 us, 34 in the form above.
 template <typename T>
 __device__ __forceinline__ void rope_rows_any(const RopeArgs& p, int block) {
   const int64_t row = block;
@@ -500,7 +501,9 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const RopeArgs p) {
 constexpr int E_MIN = -40, E_MAX = 40;  // exponents of a page scale
 constexpr float TOP_MAX = 448.0f * (1ll << E_MAX);      // the largest value that a page holds
 constexpr int MANY = 16, FEW = 4;       // rows a warp holds at once
-constexpr int SPLIT_ROWS = 1024;        // rows from which the queries get a launch of their own
+// Rows from which the queries get a launch of their own and a warp holds 16.  The host does not know the runs: prompts
+// of 1024 rows and more gain (57 against 84 us at 6,444), single rows lose (1023 take 35 us, 1024 take 127).
+constexpr int SPLIT_ROWS = 1024;
 constexpr int APPEND_THREADS = 256;
 constexpr int APPEND_WARPS = APPEND_THREADS / 32;
 
@@ -554,9 +557,12 @@ struct Window {
 // the warps' largest values meet in shared memory.  The angles of a warp's rows
 // come through shared memory, all copies in flight at once.  What bounds it is
 // latency: the chain slot -> position -> angles and row -> scale (64 single rows
-// 5.9 us, 6,600 rows of prompts 57 us, 2.6 TB/s).  With 16 rows a
+// 5.8 us, 6,444 rows of prompts in pages of 16 56 us in fp16 and 58 in bf16, 2.6
+// TB/s with the queries; 74 us in pages of 64, 82 of 128).  With 16 rows a
 // warp prompts have the most loads in flight (2 CTAs on an SM); 4 rows need half
 // the registers, and a decode step's single rows have twice the CTAs.
+// Rotary sizes that are not a multiple of 16, and unaligned rows, are read element
+// by element: 64 single rows 7.3 us, the prompts 125.
 // Every warp of the block calls it for the same run (`idle`: without an item).
 template <typename T, int EL, int ROWS, bool VEC, bool ROPE>
 __device__ __forceinline__ void append_run(const AppendArgs& p, int which, int head, int wi, bool idle, float* s_top,
@@ -916,7 +922,7 @@ int launch_append(AppendArgs& p, const hc_rope_args* rope, const hc_kv_pages* c,
   }
   // Rows a CTA searches.  Few rows: one each, since in a decode step every row is a run (1,000 single rows take
   // 35 us so, 152 us with 16 rows a warp).  Many: up to a page, for which the CTAs do not outnumber the runs so much
-  // (prompts of 6,600 rows: 57 us; 73 us when every eighth row has its CTAs).
+  // (prompts of 6,444 rows: 57 us; 73 us when every eighth row has its CTAs).
   p.seg = ROWS == FEW ? 1 : max(1, min(min(32, c->page_size), p.n_rows / 256));
   // Warps of an item.  Many rows: enough to hold a whole page.  Few: a run may be one row or a page, and the host
   // does not know which; more warps shorten long runs and make single rows wait.  8 heads, with 1, 2, 4, 8 warps:
@@ -931,7 +937,7 @@ int launch_append(AppendArgs& p, const hc_rope_args* rope, const hc_kv_pages* c,
   const int groups = (2 * p.n_kv + items - 1) / items;
   const int64_t n_append = (int64_t)((p.n_rows + p.seg - 1) / p.seg) * groups;
   // Few rows: one launch does both.  Many: the queries' rotation needs half of the registers that the write
-  // does, and runs faster as a kernel of its own, which the write may run beside (6,600 rows of prompts with 32
+  // does, and runs faster as a kernel of its own, which the write may run beside (6,444 rows of prompts with 32
   // query heads: 57 us, 84 in one launch).
   if (rope && ROWS == MANY) {
     if (vec) rope_kernel<T, true><<<(unsigned)extra, ROPE_THREADS, 0, stream>>>(ra);

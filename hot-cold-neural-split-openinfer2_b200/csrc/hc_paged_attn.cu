@@ -19,11 +19,14 @@
 // 2^-36 of that one at most below (W_REF in hc_paged_attn.cuh); a row of many
 // small weights beside one large one needs that room.
 //
-// Bound by HBM, each cached byte read once: 4 requests of 60,000 to 131,000
-// keys, 32 / 8 heads of 128, 134 us (5.8 TB/s; a copy of this loop that only
-// loads takes 132); 64 requests of 100 to 8000 keys 96 us (5.6 TB/s).  Three
-// CTAs of four warps on an SM; two, eight warps each, were slower, and so were
-// shares of a half or a quarter of this length (more items are cut).
+// Bound by HBM, each cached byte read once (in a graph; 32 / 8 heads of 128): 4
+// requests of 60,000 to 131,000 keys 134 to 141 us by the run (5.5 to 5.8 TB/s; a
+// copy of this loop that only loads takes 132); 64 requests of 100 to 8000 keys
+// 96 to 99 us (5.4 to 5.6 TB/s).  With 9 to 16 rows an item (NT = 2) the latter
+// take 129 us: 232 registers leave two CTAs an SM, and with them a third fewer
+// loads in flight (HBM at 53% of its peak, 70% with NT = 1).  Three CTAs of four
+// warps on an SM; two, eight warps each, were slower, and so were shares of a
+// half or a quarter of this length (more items are cut).
 #include "hc_paged_attn.cuh"
 
 namespace hca8 {
@@ -34,7 +37,7 @@ constexpr int WARPS = THREADS / 32;
 constexpr int STAGES = 3;              // chunks in flight per warp
 constexpr int ITEM_COST = 16;          // what beginning an item costs, in chunks
 // Rows of a request and head that these kernels take: two MMA columns of 8.  64 requests of 100 to 8000 keys with
-// 16 rows take 129 us here; with 20 rows the tiles of hc_paged_prefill.cu take 274 us, and as much for fewer.
+// 16 rows take 129 us here; with 20 rows the tiles of hc_paged_prefill.cu take 276 us, with 64 rows 280.
 constexpr int SMALL = 16;
 constexpr int MIN_SHARE = 2 * WARPS;   // units of a share at least
 
@@ -610,7 +613,8 @@ int launch(AttnParams& p, void* workspace, cudaStream_t stream) {
 
 template <typename T>
 int launch_typed(AttnParams& p, int head_dim, int rows, void* workspace, cudaStream_t stream) {
-  // rows of a request and head: 8 fill one MMA's columns (64 requests as above 99 us), more take two (128 us)
+  // rows of the largest request and head: 8 fill one MMA's columns (64 requests as above 99 us), more take two
+  // (129 us).  A step that holds both, or prompts beside single tokens, runs its small requests on the latter too.
   if (head_dim == 128)
     return rows <= 8 ? launch<T, 128, 1>(p, workspace, stream) : launch<T, 128, 2>(p, workspace, stream);
   return rows <= 8 ? launch<T, 64, 1>(p, workspace, stream) : launch<T, 64, 2>(p, workspace, stream);

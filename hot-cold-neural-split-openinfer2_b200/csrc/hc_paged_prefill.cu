@@ -17,14 +17,17 @@
 // MIN_PIECE); the pieces of a cut tile leave partial softmaxes, which a second
 // kernel joins.
 //
-// What bounds it: issue slots and the exponentials, which the softmax warps, the
-// converters and the products' issuers share on four schedulers.  A prompt of
-// 4096 tokens, 32 / 8 heads of 128: 157 us, 874 TFLOP/s (the products alone need
-// 86 us, its exponentials 62 at half of that for dim 64).  Pieces of 33 to 1500
-// tokens behind up to 8000, 16 / 2 heads of 64: 160 us; 64 rows behind 30,000
-// keys 70 us, 1.6 ms if their keys are not cut.  A converted tile serves 256
-// rows: 8 converter warps at 96 registers took 167 us for the prompt, tiles
-// converted 64 keys at a time 164.
+// What bounds it: the latency of a half's chain (score barrier, TMEM loads,
+// maximum, exponentials, TMEM stores, barrier), which two softmax warps a
+// scheduler do not cover.  No resource is busy all the time: at dim 128 the tensor
+// pipe 43%, the exponentials' 44%, issue slots 45%; at dim 64 26, 53 and 44%.  A
+// prompt of 4096 tokens, 32 / 8 heads of 128: 155 to 157 us in a graph, 880
+// TFLOP/s, 164 as a call among others (the products alone need 86 us).  Pieces of
+// 33 to 1500 tokens behind up to 8000, 16 / 2 heads of 64: 160 us, of which 45 are
+// products and 62 exponentials; their 220 unequal units on 148 SMs leave a tail.
+// 16 tokens of 4 heads a group behind 30,000 keys 57 us, 1.6 ms if their keys are
+// not cut.  A converted tile serves 256 rows: 8 converter warps at 96 registers
+// took 167 us for the prompt, tiles converted 64 keys at a time 164.
 //
 // Page scales: a key's scale joins the factor of its 16 score columns, a
 // value's scale enters as log2 in the exponent (see hc_paged_attn.cu).
@@ -836,7 +839,7 @@ __global__ void __launch_bounds__(ROWS) paged_prefill_join_kernel(const AttnPara
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const float4 v = reinterpret_cast<const float4*>(q)[(4 * blockIdx.y + c) * ROWS + t];
-        // a piece that the row sees nothing of adds nothing, whatever its sums hold
+        // a piece that the row sees nothing of has f = 0; its sums are finite, as the cache holds no NaN
         a[4 * c] = fmaf(v.x, f, a[4 * c]);
         a[4 * c + 1] = fmaf(v.y, f, a[4 * c + 1]);
         a[4 * c + 2] = fmaf(v.z, f, a[4 * c + 2]);

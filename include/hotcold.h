@@ -591,7 +591,8 @@ HC_API int hc_page_plan(const int32_t* starts, const int32_t* q_lens, int32_t n_
  * hc_page_release -- the pages of every request with done[r] != 0 go back
  * onto the stack and its table row becomes missing (-1).  More pages than
  * n_pages in all, an id not below n_pages, or a page behind a missing one:
- * HC_ERR_RANGE and nothing is released.  A page shared by two tables is not known here: release one.
+ * HC_ERR_RANGE and nothing is released.  A page shared by two tables is not
+ * known here: release one.
  */
 HC_API int hc_page_release(const uint8_t* done, int32_t n_requests, int32_t* tables, int64_t table_stride,
                            int32_t table_width, int32_t* free_pages, int32_t n_pages, int32_t* n_free,
@@ -677,7 +678,11 @@ HC_API int hc_rope_append(const hc_rope_args* args, const hc_kv_pages* cache, co
  *              can overlap)
  * Softmax statistics are fp32; a page id outside the cache, a length past the
  * table or rows past n_rows set HC_ERR_RANGE and are left out.  Bytes of
- * positions behind kv_lens are never used, whatever they hold.
+ * positions behind kv_lens are never used, whatever they hold; those before
+ * are numbers, as hc_kv_append writes them (a NaN value would reach the rows
+ * of a step in front of it, too).  Weights are rounded to f16 for the product:
+ * 2^-11 relative down to 2^-25 of a row's largest weight times value scale,
+ * and by 2^-36 of that at most below.
  * A request whose offsets go back is left out with HC_ERR_RANGE, too; when
  * such offsets make the others of more than 16 rows a key-value head claim more
  * rows than n_rows, none of those is served.
